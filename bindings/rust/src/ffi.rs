@@ -48,6 +48,14 @@ pub const SLHIP_NEG_DIV: i32 = 7;
 pub const SLHIP_TANH: i32 = 8;
 pub const SLHIP_SIGMOID: i32 = 9;
 
+/// Activation codes of slhip_group_norm and forms of slhip_gated_scan.
+pub const SLHIP_ACT_NONE: i32 = 0;
+pub const SLHIP_ACT_RELU: i32 = 1;
+pub const SLHIP_ACT_SILU: i32 = 2;
+pub const SLHIP_ACT_GELU: i32 = 3;
+pub const SLHIP_SCAN_LINEAR: i32 = 0;
+pub const SLHIP_SCAN_SIGMOID: i32 = 1;
+
 pub const SLHIP_TAIL_AUTO: i32 = 0;
 pub const SLHIP_TAIL_WHOLE: i32 = 1;
 pub const SLHIP_TAIL_SPREAD: i32 = 2;
@@ -383,6 +391,102 @@ extern "C" {
         grads: *const *const f32,
         lens: *const usize,
         lr: f32,
+    ) -> i32;
+    pub fn slhip_adamw_step_multi(
+        ctx: *mut SlhipCtx,
+        count: usize,
+        params: *const *mut f32,
+        grads: *const *const f32,
+        m: *const *mut f32,
+        v: *const *mut f32,
+        lens: *const usize,
+        lr: f32,
+        beta1: f32,
+        beta2: f32,
+        eps: f32,
+        weight_decay: f32,
+        step: u64,
+        step_dev: *mut u64,
+    ) -> i32;
+    pub fn slhip_adamw8_step_multi(
+        ctx: *mut SlhipCtx,
+        count: usize,
+        params: *const *mut f32,
+        grads: *const *const f32,
+        m8: *const *mut c_void,
+        v8: *const *mut c_void,
+        scales: *const *mut f32,
+        lens: *const usize,
+        lr: f32,
+        beta1: f32,
+        beta2: f32,
+        eps: f32,
+        weight_decay: f32,
+        step: u64,
+        step_dev: *mut u64,
+        seed: u64,
+    ) -> i32;
+    pub fn slhip_group_norm(
+        ctx: *mut SlhipCtx,
+        samples: usize,
+        positions: usize,
+        channels: usize,
+        groups: usize,
+        act: i32,
+        eps: f32,
+        x: *const f32,
+        weight: *const f32,
+        bias: *const f32,
+        mean: *mut f32,
+        rstd: *mut f32,
+        out: *mut f32,
+    ) -> i32;
+    pub fn slhip_group_norm_grad(
+        ctx: *mut SlhipCtx,
+        samples: usize,
+        positions: usize,
+        channels: usize,
+        groups: usize,
+        act: i32,
+        x: *const f32,
+        weight: *const f32,
+        bias: *const f32,
+        mean: *const f32,
+        rstd: *const f32,
+        x_grad: *mut f32,
+        weight_grad: *mut f32,
+        bias_grad: *mut f32,
+        out_grad: *const f32,
+        beta: f32,
+    ) -> i32;
+    pub fn slhip_gated_scan(
+        ctx: *mut SlhipCtx,
+        mode: i32,
+        batch: usize,
+        steps: usize,
+        channels: usize,
+        gate: *const f32,
+        x: *const f32,
+        h0: *const f32,
+        h: *mut f32,
+        h_last: *mut f32,
+    ) -> i32;
+    pub fn slhip_gated_scan_grad(
+        ctx: *mut SlhipCtx,
+        mode: i32,
+        batch: usize,
+        steps: usize,
+        channels: usize,
+        gate: *const f32,
+        x: *const f32,
+        h0: *const f32,
+        h: *const f32,
+        gate_grad: *mut f32,
+        x_grad: *mut f32,
+        h0_grad: *mut f32,
+        h_grad: *const f32,
+        h_last_grad: *const f32,
+        beta: f32,
     ) -> i32;
     pub fn slhip_cce(
         ctx: *mut SlhipCtx,

@@ -243,6 +243,53 @@ int32_t slhip_softmax(slhip_ctx* ctx, size_t samples, size_t features, const flo
 int32_t slhip_softmax_grad(slhip_ctx* ctx, size_t samples, size_t features, float* x_grad,
                            const float* out, const float* out_grad, float beta);
 
+/* ---------------------------------------------------------------- group norm -------
+ * Group normalisation with an activation, channels last: x is samples × positions × channels, row-major,
+ * the channels in `groups` runs of equal length (groups divides channels).  No counterpart in the
+ * reference.  Over each sample's group, m = positions · channels/groups values:
+ *     mean, rstd = 1/sqrt(var + eps);  u = (x − mean)·rstd·weight[c] + bias[c];  out = act(u)
+ * groups = 1 and positions = 1 is a layer norm of every row.  weight and bias (channels each) may be
+ * NULL (ones, zeros).  mean and rstd (samples × groups each) receive what the backward pass needs and
+ * may be NULL.  out may alias x.
+ * slhip_group_norm_grad, with g = out_grad ⊙ act'(u), hat = (x − mean)·rstd, gx = g·weight, < > a mean over the
+ * sample's group:
+ *     x_grad      = beta·x_grad + rstd·(gx − <gx> − hat·<gx·hat>)
+ *     weight_grad = beta·weight_grad + Σ g·hat      bias_grad = beta·bias_grad + Σ g
+ * beta 0 = SET, 1 = accumulate.  x_grad, weight_grad and bias_grad may each be NULL (skipped); x_grad may
+ * alias out_grad.  Every sum has a fixed order.  SLHIP_ACT_GELU is x·Φ(x) with the error function, relu'
+ * is (u >= 0) as everywhere here. */
+enum { SLHIP_ACT_NONE = 0, SLHIP_ACT_RELU = 1, SLHIP_ACT_SILU = 2, SLHIP_ACT_GELU = 3 };
+int32_t slhip_group_norm(slhip_ctx* ctx, size_t samples, size_t positions, size_t channels, size_t groups, int32_t act,
+                         float eps, const float* x, const float* weight, const float* bias, float* mean, float* rstd,
+                         float* out);
+int32_t slhip_group_norm_grad(slhip_ctx* ctx, size_t samples, size_t positions, size_t channels, size_t groups, int32_t act,
+                              const float* x, const float* weight, const float* bias, const float* mean, const float* rstd,
+                              float* x_grad, float* weight_grad, float* bias_grad, const float* out_grad, float beta);
+
+/* ---------------------------------------------------------------- gated recurrence --
+ * The linear recurrence of a gated recurrent layer along `steps`, every channel for itself; gate, x and h are
+ * batch × steps × channels, row-major.  No counterpart in the reference.
+ *     SLHIP_SCAN_LINEAR   h_t = gate_t·h_{t−1} + x_t
+ *     SLHIP_SCAN_SIGMOID  h_t = s·h_{t−1} + (1 − s)·x_t,  s = 1/(1 + exp(−gate_t))
+ * h_{−1} is h0 (batch × channels; NULL: zeros).  h_last (may be NULL) receives h_{steps−1}, the h0 of a call that
+ * goes on from here - steps = 1 is one token of a serving loop - and may be h0 itself.  h may alias x
+ * or gate when it is the same array.
+ * Long sequences are cut into runs that are joined by their products of gates, in a fixed order.  For
+ * SLHIP_SCAN_LINEAR a product of gates over a run of steps has to be representable: gates of magnitude
+ * up to one always are.
+ * slhip_gated_scan_grad: with h_grad (and h_last_grad, which may be NULL) given and h as the forward call left it,
+ * d_t = h_grad_t + a_{t+1}·d_{t+1} (a = gate or s; d_{steps-1} also takes h_last_grad):
+ *     LINEAR   gate_grad = d·h_{t−1}                   x_grad = d
+ *     SIGMOID  gate_grad = d·(h_{t−1} − x)·s·(1 − s)      x_grad = d·(1 − s)         h0_grad = a_0·d_0
+ * each beta·(old value) + that; each may be NULL (skipped), and none may overlap an input.  x may be NULL
+ * for SLHIP_SCAN_LINEAR. */
+enum { SLHIP_SCAN_LINEAR = 0, SLHIP_SCAN_SIGMOID = 1 };
+int32_t slhip_gated_scan(slhip_ctx* ctx, int32_t mode, size_t batch, size_t steps, size_t channels, const float* gate,
+                         const float* x, const float* h0, float* h, float* h_last);
+int32_t slhip_gated_scan_grad(slhip_ctx* ctx, int32_t mode, size_t batch, size_t steps, size_t channels, const float* gate,
+                              const float* x, const float* h0, const float* h, float* gate_grad, float* x_grad,
+                              float* h0_grad, const float* h_grad, const float* h_last_grad, float beta);
+
 /* ---------------------------------------------------------------- transpose --------
  * Transpose::transpose(rows, cols, x) (src/ops2/transpose/mod.rs:17-21; slice_transpose
  * src/ops2/transpose/cpu.rs:10-25): out[c·rows + r] = x[r·cols + c].  beta 0 = `Set`, 1 = `Assign`
@@ -335,6 +382,31 @@ int32_t slhip_sgd_step(slhip_ctx* ctx, size_t n, float* p, const float* g, float
  * arrays of `count` device pointers / lengths. */
 int32_t slhip_sgd_step_multi(slhip_ctx* ctx, size_t count, float* const* params, const float* const* grads,
                              const size_t* lens, float lr);
+/* AdamW for `count` parameter tensors, in one launch per 64 tensors (beside slhip_sgd_step_multi; the
+ * reference's examples train by SGD only).  With t the number of the step:
+ *     m = beta1·m + (1 − beta1)·g          v = beta2·v + (1 − beta2)·g·g
+ *     p = p·(1 − lr·weight_decay) − lr/(1 − beta1^t) · m / (sqrt(v)/sqrt(1 − beta2^t) + eps)
+ * params, grads, m, v and lens are HOST arrays of `count` device pointers / lengths; the moments start
+ * as zeros.  t is `step`, counted from 1; or, with step = 0, the counter that step_dev (a device
+ * pointer, 8-byte aligned, starting at zero) names, which the call advances by one first: that is the
+ * form for recorded steps, whose replays must not repeat one t (one more small launch, which leaves
+ * what it computes in the workspace).  No two tensors may overlap (SLHIP_EALIAS), nor a gradient any
+ * array that is written.  beta1 and beta2 lie in [0, 1), eps >= 0.
+ * slhip_adamw8_step_multi keeps the moments in 8 bits: m8[i] holds lens[i] OCP E4M3 values, v8[i] lens[i]
+ * OCP E5M2 values (both 4-byte aligned), and scales[i] two floats, m's and v's, for every started block
+ * of 256 elements; a moment is its 8-bit value times its block's scale, a power of two.  All start as
+ * zeros.  The update uses the moments before they are rounded.  m is rounded to nearest, v
+ * stochastically (rounded to nearest, a decay of 0.1 % a step would never leave the spacing of 8 bits),
+ * with random bits that depend on seed, t, the tensor's place in the list and the element alone; a v
+ * that is not zero never rounds to zero.  Infinite and NaN moments stay in their own element (E4M3 has no
+ * infinity: an infinite m is kept as NaN). */
+int32_t slhip_adamw_step_multi(slhip_ctx* ctx, size_t count, float* const* params, const float* const* grads,
+                               float* const* m, float* const* v, const size_t* lens, float lr, float beta1, float beta2,
+                               float eps, float weight_decay, uint64_t step, uint64_t* step_dev);
+int32_t slhip_adamw8_step_multi(slhip_ctx* ctx, size_t count, float* const* params, const float* const* grads,
+                                void* const* m8, void* const* v8, float* const* scales, const size_t* lens, float lr,
+                                float beta1, float beta2, float eps, float weight_decay, uint64_t step, uint64_t* step_dev,
+                                uint64_t seed);
 int32_t slhip_cce(slhip_ctx* ctx, size_t rows, size_t cols, const float* preds, const float* targets, float* loss);
 int32_t slhip_cce_grad(slhip_ctx* ctx, size_t rows, size_t cols, const float* preds, const float* targets,
                        float* grad);

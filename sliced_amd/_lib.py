@@ -97,6 +97,14 @@ PROTOTYPES = {
     "slhip_softmax_cce_grad": [c_vp, c_sz, c_sz, c_vp, c_vp, c_vp, C.c_float, c_vp],
     "slhip_mlp3_mse_step": [c_vp, c_sz, c_sz, c_sz, c_sz, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, C.c_float, c_vp],
     "slhip_sgd_step_multi": [c_vp, c_sz, c_vp, c_vp, c_vp, C.c_float],
+    "slhip_adamw_step_multi": [c_vp, c_sz, c_vp, c_vp, c_vp, c_vp, c_vp, C.c_float, C.c_float, C.c_float, C.c_float, C.c_float,
+                               C.c_uint64, c_vp],
+    "slhip_adamw8_step_multi": [c_vp, c_sz, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, C.c_float, C.c_float, C.c_float, C.c_float,
+                                C.c_float, C.c_uint64, c_vp, C.c_uint64],
+    "slhip_group_norm": [c_vp, c_sz, c_sz, c_sz, c_sz, c_i32, C.c_float, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp],
+    "slhip_group_norm_grad": [c_vp, c_sz, c_sz, c_sz, c_sz, c_i32, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, C.c_float],
+    "slhip_gated_scan": [c_vp, c_i32, c_sz, c_sz, c_sz, c_vp, c_vp, c_vp, c_vp, c_vp],
+    "slhip_gated_scan_grad": [c_vp, c_i32, c_sz, c_sz, c_sz, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, c_vp, C.c_float],
     "slhip_cce": [c_vp, c_sz, c_sz, c_vp, c_vp, c_vp],
     "slhip_cce_grad": [c_vp, c_sz, c_sz, c_vp, c_vp, c_vp],
     "slhip_onehot": [c_vp, c_sz, c_sz, c_vp, c_vp],

@@ -79,6 +79,31 @@ int32_t hip_fail(hipError_t e, const char* what);
     }                                                           \
   } while (0)
 
+// Makes the context's device current for the length of a call, and the caller's current again after it:
+// a thread may drive contexts of several devices, and a launch goes to the current one.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    if (hipGetDevice(&before_) != hipSuccess) before_ = device;
+    if (before_ != device) status_ = hipSetDevice(device);
+    changed_ = before_ != device && status_ == hipSuccess;
+  }
+  ~OnDevice() {
+    if (changed_) (void)hipSetDevice(before_);
+  }
+  OnDevice(const OnDevice&) = delete;
+  OnDevice& operator=(const OnDevice&) = delete;
+  hipError_t status() const { return status_; }
+
+ private:
+  int before_ = 0;
+  bool changed_ = false;
+  hipError_t status_ = hipSuccess;
+};
+#define SLHIP_ON_DEVICE(ctx)                  \
+  slhip::OnDevice on_device_((ctx)->device);  \
+  SLHIP_CHECK_HIP(on_device_.status())
+
 // rows*cols with overflow check; false on overflow or zero.
 inline bool checked_len(size_t rows, size_t cols, size_t* len) {
   if (rows == 0 || cols == 0) return false;

@@ -44,10 +44,16 @@ class Buf:
 
 
 class Context:
-    def __init__(self, ordinal=0):
+    """A context of its own stream, or, with `stream` (a hipStream_t as an integer, 0 for the default
+    stream), one that issues its ops on that stream."""
+
+    def __init__(self, ordinal=0, stream=None):
         self.lib = _lib.load()
         h = C.c_void_p()
-        _lib.check(self.lib.slhip_init(ordinal, C.byref(h)), "slhip_init")
+        if stream is None:
+            _lib.check(self.lib.slhip_init(ordinal, C.byref(h)), "slhip_init")
+        else:
+            _lib.check(self.lib.slhip_init_on_stream(ordinal, stream, C.byref(h)), "slhip_init_on_stream")
         self.h = h
         self._bufs = []
 

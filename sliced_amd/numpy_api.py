@@ -610,3 +610,86 @@ def rand_uniform(n, lo, hi, tag, seed):
         b = s.c.uniform(n, lo, hi, tag, seed)
         s.bufs.append(b)
         return b.numpy()
+
+
+# ---- group norm, gated recurrence, AdamW --------------------------------------
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = range(4)
+SCAN_LINEAR, SCAN_SIGMOID = 0, 1
+
+
+def group_norm(samples, positions, channels, groups, x, weight=None, bias=None, act=ACT_NONE, eps=1e-5):
+    """(out, mean, rstd) of slhip_group_norm; mean and rstd have samples * groups values"""
+    with _Scope() as s:
+        dx, dw, db = s.up(x), s.up(weight), s.up(bias)
+        dm, dr, do = s.empty(samples * groups), s.empty(samples * groups), s.empty(samples * positions * channels)
+        s.c.call("slhip_group_norm", samples, positions, channels, groups, act, eps, dx.ptr, _ptr(dw), _ptr(db), dm.ptr, dr.ptr, do.ptr)
+        return do.numpy(), dm.numpy(), dr.numpy()
+
+
+def group_norm_grad(samples, positions, channels, groups, x, weight, bias, mean, rstd, out_grad, x_grad, weight_grad, bias_grad,
+                    act=ACT_NONE, beta=0.0):
+    """slhip_group_norm_grad; each of the three gradients is updated in place, or left out where it is None"""
+    with _Scope() as s:
+        dx, dw, db, dm, dr, dg = s.up(x), s.up(weight), s.up(bias), s.up(mean), s.up(rstd), s.up(out_grad)
+        outs = [s.up(g) for g in (x_grad, weight_grad, bias_grad)]
+        s.c.call("slhip_group_norm_grad", samples, positions, channels, groups, act, dx.ptr, _ptr(dw), _ptr(db), dm.ptr, dr.ptr,
+                 *[_ptr(o) for o in outs], dg.ptr, float(beta))
+        for host, dev in zip((x_grad, weight_grad, bias_grad), outs):
+            if host is not None:
+                host[:] = dev.numpy()
+
+
+def gated_scan(mode, batch, steps, channels, gate, x, h0=None):
+    """(h, h_last) of slhip_gated_scan"""
+    with _Scope() as s:
+        dg, dx, d0 = s.up(gate), s.up(x), s.up(h0)
+        dh, dl = s.empty(batch * steps * channels), s.empty(batch * channels)
+        s.c.call("slhip_gated_scan", mode, batch, steps, channels, dg.ptr, dx.ptr, _ptr(d0), dh.ptr, dl.ptr)
+        return dh.numpy(), dl.numpy()
+
+
+def gated_scan_grad(mode, batch, steps, channels, gate, x, h0, h, h_grad, gate_grad, x_grad, h0_grad, h_last_grad=None, beta=0.0):
+    """slhip_gated_scan_grad; each of the three gradients is updated in place, or left out where it is None"""
+    with _Scope() as s:
+        dg, dx, d0, dh, dd, dl = (s.up(a) for a in (gate, x, h0, h, h_grad, h_last_grad))
+        outs = [s.up(g) for g in (gate_grad, x_grad, h0_grad)]
+        s.c.call("slhip_gated_scan_grad", mode, batch, steps, channels, dg.ptr, _ptr(dx), _ptr(d0), dh.ptr, *[_ptr(o) for o in outs],
+                 dd.ptr, _ptr(dl), float(beta))
+        for host, dev in zip((gate_grad, x_grad, h0_grad), outs):
+            if host is not None:
+                host[:] = dev.numpy()
+
+
+def _pointers(bufs):
+    return (C.c_void_p * len(bufs))(*[b.ptr for b in bufs])
+
+
+def adamw_step_multi(params, grads, m, v, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, step=1):
+    """slhip_adamw_step_multi on lists of arrays; params, m and v are updated in place"""
+    with _Scope() as s:
+        dev = [[s.up(a) for a in arrays] for arrays in (params, grads, m, v)]
+        lens = (C.c_size_t * len(params))(*[p.size for p in params])
+        s.c.call("slhip_adamw_step_multi", len(params), *[_pointers(d) for d in dev], lens, lr, beta1, beta2, eps, weight_decay, step, None)
+        for host, d in ((params, dev[0]), (m, dev[2]), (v, dev[3])):
+            for a, b in zip(host, d):
+                a[:] = b.numpy().reshape(a.shape)
+
+
+def adamw8_step_multi(params, grads, m8, v8, scales, lr, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, step=1, seed=0):
+    """slhip_adamw8_step_multi on lists of arrays: m8 and v8 are uint8 (the E4M3 and E5M2 codes), scales has two floats
+    for every started block of 256 elements; all but the gradients are updated in place"""
+    def words(a):                                  # bytes travel as whole floats, the last one padded
+        return np.concatenate([a, np.zeros(-a.size % 4, np.uint8)]).view(np.float32)
+
+    with _Scope() as s:
+        dp, dg, ds = ([s.up(a) for a in arrays] for arrays in (params, grads, scales))
+        dm, dv = ([s.up(words(a)) for a in arrays] for arrays in (m8, v8))
+        lens = (C.c_size_t * len(params))(*[p.size for p in params])
+        s.c.call("slhip_adamw8_step_multi", len(params), *[_pointers(d) for d in (dp, dg, dm, dv, ds)], lens, lr, beta1, beta2, eps,
+                 weight_decay, step, None, seed)
+        for host, dev in ((params, dp), (scales, ds)):
+            for a, b in zip(host, dev):
+                a[:] = b.numpy().reshape(a.shape)
+        for host, dev in ((m8, dm), (v8, dv)):
+            for a, b in zip(host, dev):
+                a[:] = b.numpy().view(np.uint8)[:a.size]
