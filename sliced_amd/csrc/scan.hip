@@ -62,6 +62,17 @@ __device__ __forceinline__ void scan_store(float* p, const ScanVec<V>& r, int nv
     if (k < nv) p[k] = r.v[k];
 }
 
+// p = beta * p + r
+template <int V>
+__device__ __forceinline__ void scan_grad_store(float* p, ScanVec<V> r, int nv, float beta) {
+  if (beta != 0.0f) {
+    const ScanVec<V> old = scan_load<V>(p, nv, 0.0f);
+#pragma unroll
+    for (int k = 0; k < V; ++k) r.v[k] = beta * old.v[k] + r.v[k];
+  }
+  scan_store<V>(p, r, nv);
+}
+
 // s and 1 - s of a sigmoid, each to a few units in its last place at either end: e = exp(-|z|) never
 // overflows, and the smaller of the two is e / (1 + e), not a difference.
 __device__ __forceinline__ void scan_sigmoid(float z, float& s, float& rest) {
@@ -165,36 +176,346 @@ __global__ __launch_bounds__(256) void scan_rows_grad_kernel(ScanArgs a) {
           dg.v[k] = (dxv.v[k] * s) * (before[r].v[k] - x[r].v[k]);
         }
       }
-      if (a.dgate) {
-        if (a.beta != 0.0f) {
-          const ScanVec<V> old = scan_load<V>(a.dgate + row, nv, 0.0f);
+      if (a.dgate) scan_grad_store<V>(a.dgate + row, dg, nv, a.beta);
+      if (a.dx) scan_grad_store<V>(a.dx + row, dxv, nv, a.beta);
+    }
+  }
+  if (a.dh0) scan_grad_store<V>(a.dh0 + state, G, nv, a.beta);
+}
+
+// ---------------------------------------------------------------- many steps at a time
+// A workgroup owns L * V channels and takes NT / L runs of R steps of them at a time, a run to a thread.  A thread
+// folds its run to a pair (A, H) - the run takes a state s to A s + H - the pairs are joined across the workgroup, and with
+// the state that then reaches its run a thread goes through it again, out of registers.  The next tile's loads are in
+// flight meanwhile.  Nothing is read twice.
+//
+// Where that leaves the chip idle (few channels, many steps) the steps are also split into chunks over workgroups:
+// scan_totals_kernel finds every chunk's pair, and each workgroup then joins those before its own.  That reads the
+// inputs of the recurrence a second time; the joins go through the workspace.
+struct ScanSplit {
+  size_t chunk;    // steps of a workgroup
+  float* pairs;    // [chunks - 1][batch][2][channels]
+  float* h0;       // the initial state as it was before h_last, which may be the same array, is written
+};
+
+// What a thread holds of a run of R steps.
+template <bool GRAD, int MODE, int V, int R>
+struct ScanRun {
+  ScanVec<V> g[R];
+  ScanVec<V> x[GRAD && MODE == SLHIP_SCAN_LINEAR ? 1 : R];
+  ScanVec<V> dh[GRAD ? R : 1];
+  ScanVec<V> before[GRAD ? R : 1];
+};
+
+// Where a thread's channels and its workgroup's chunk of steps lie.  Steps are counted in running order: u = t forward,
+// u = steps - 1 - t backward.
+template <int V, int L>
+struct ScanPlace {
+  size_t b, c, u0, u1;
+  int nv;
+  __device__ __forceinline__ ScanPlace(const ScanArgs& a, const ScanSplit& s, unsigned chunk) {
+    const size_t tiles = (a.channels + L * V - 1) / (L * V);
+    b = blockIdx.x / tiles;
+    c = ((blockIdx.x - b * tiles) * L + threadIdx.x % L) * V;
+    nv = c >= a.channels ? 0 : a.channels - c < (size_t)V ? (int)(a.channels - c) : V;
+    u0 = chunk * s.chunk;
+    u1 = u0 + s.chunk < a.steps ? u0 + s.chunk : a.steps;
+  }
+};
+
+// Rows of R steps from u on, those at and past `end` replaced by the step before it (they are masked later).
+template <bool GRAD, int V, int R>
+__device__ __forceinline__ void scan_load_rows(ScanVec<V>* out, const float* src, const ScanArgs& a, size_t b, size_t c, int nv, size_t u,
+                                               size_t end) {
+  const size_t first = u < end ? u : end - 1, left = end - first;
+  const float* at = src + (b * a.steps + (GRAD ? a.steps - 1 - first : first)) * a.channels + c;
+  if (V == 4 && nv == 4) {
 #pragma unroll
-          for (int k = 0; k < V; ++k) dg.v[k] = a.beta * old.v[k] + dg.v[k];
-        }
-        scan_store<V>(a.dgate + row, dg, nv);
+    for (int r = 0; r < R; ++r) {
+      const size_t o = ((size_t)r < left ? (size_t)r : left - 1) * a.channels;
+      out[r] = scan_load<V>(GRAD ? at - o : at + o, V, 0.0f);
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const size_t o = ((size_t)r < left ? (size_t)r : left - 1) * a.channels;
+#pragma unroll
+      for (int k = 0; k < V; ++k) out[r].v[k] = k < nv ? (GRAD ? at - o : at + o)[k] : 0.0f;
+    }
+  }
+}
+
+template <bool GRAD, int MODE, int V, int R>
+__device__ __forceinline__ void scan_load_run(ScanRun<GRAD, MODE, V, R>& run, const ScanArgs& a, size_t b, size_t c, int nv, size_t u,
+                                              size_t end) {
+  scan_load_rows<GRAD, V, R>(run.g, a.gate, a, b, c, nv, u, end);
+  if (!GRAD) {
+    scan_load_rows<GRAD, V, R>(run.x, a.x, a, b, c, nv, u, end);
+    return;
+  }
+  scan_load_rows<GRAD, V, GRAD ? R : 1>(run.dh, a.dh, a, b, c, nv, u, end);
+  if (MODE == SLHIP_SCAN_SIGMOID) scan_load_rows<GRAD, V, GRAD && MODE == SLHIP_SCAN_LINEAR ? 1 : R>(run.x, a.x, a, b, c, nv, u, end);
+  // h one step earlier; before the first step the initial state
+  const size_t first = u < end ? u : end - 1, left = end - first, row = a.steps - 1 - first;
+#pragma unroll
+  for (int r = 0; r < (GRAD ? R : 1); ++r) {
+    const size_t o = (size_t)r < left ? (size_t)r : left - 1;
+    const float* src = row > o ? a.h + (b * a.steps + row - o - 1) * a.channels + c : a.h0 ? a.h0 + b * a.channels + c : nullptr;
+    run.before[r] = scan_load<V>(src, src ? nv : 0, 0.0f);
+  }
+}
+
+// Folds R steps from u on into (A, H): coefficients co and inputs in stay for the second pass.
+template <bool GRAD, int MODE, int V, int R>
+__device__ __forceinline__ void scan_fold(const ScanVec<V>* g, const ScanVec<V>* x, size_t u, size_t end, ScanVec<V>* co, ScanVec<V>* in,
+                                          ScanVec<V>& A, ScanVec<V>& H) {
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const bool some = u + r < end;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      float c, i, rest = 0.0f;
+      if (GRAD) {
+        c = g[r].v[k];
+        if (MODE == SLHIP_SCAN_SIGMOID) scan_sigmoid(g[r].v[k], c, rest);
+        c = some ? c : 1.0f;
+        i = some ? x[r].v[k] : 0.0f;                 // dh; what enters is c * dh
+        H.v[k] = some ? c * (H.v[k] + i) : H.v[k];
+        in[r].v[k] = rest;
+      } else {
+        c = scan_coefficient<MODE>(g[r].v[k], x[r].v[k], i);
+        c = some ? c : 1.0f;
+        i = some ? i : 0.0f;
+        H.v[k] = some ? fmaf(c, H.v[k], i) : H.v[k];
+        in[r].v[k] = i;
       }
-      if (a.dx) {
-        if (a.beta != 0.0f) {
-          const ScanVec<V> old = scan_load<V>(a.dx + row, nv, 0.0f);
+      co[r].v[k] = c;
+      A.v[k] *= c;
+    }
+  }
+}
+
+// Joins the threads' pairs in the order of their runs: replaces (A, H) by the inclusive pairs within the wave and leaves the
+// waves' in LDS, `totals`, for after the next barrier.
+template <int V, int L>
+__device__ __forceinline__ void scan_join_wave(ScanVec<V>& A, ScanVec<V>& H, float (*totals)[2][L * V]) {
+  const int lane = threadIdx.x & 63, run = lane / L;
 #pragma unroll
-          for (int k = 0; k < V; ++k) dxv.v[k] = a.beta * old.v[k] + dxv.v[k];
-        }
-        scan_store<V>(a.dx + row, dxv, nv);
+  for (int d = 1; d < 64 / L; d *= 2) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      const float pa = __shfl_up(A.v[k], d * L, WAVE), ph = __shfl_up(H.v[k], d * L, WAVE);
+      if (run >= d) {
+        H.v[k] = fmaf(A.v[k], ph, H.v[k]);
+        A.v[k] *= pa;
       }
     }
   }
-  if (a.dh0) {
-    if (a.beta != 0.0f) {
-      const ScanVec<V> old = scan_load<V>(a.dh0 + state, nv, 0.0f);
+  if (run == 64 / L - 1) {
+    const int w = threadIdx.x >> 6, l = lane % L;
 #pragma unroll
-      for (int k = 0; k < V; ++k) G.v[k] = a.beta * old.v[k] + G.v[k];
+    for (int k = 0; k < V; ++k) {
+      totals[w][0][l * V + k] = A.v[k];
+      totals[w][1][l * V + k] = H.v[k];
     }
-    scan_store<V>(a.dh0 + state, G, nv);
   }
+}
+// The state that reaches this thread's run; `carry` becomes the state behind all runs of the workgroup.
+template <int V, int L, int NW>
+__device__ __forceinline__ ScanVec<V> scan_reach(const ScanVec<V>& A, const ScanVec<V>& H, ScanVec<V>& carry,
+                                                 const float (*totals)[2][L * V]) {
+  const int lane = threadIdx.x & 63, run = lane / L, l = lane % L, wave = threadIdx.x >> 6;
+  ScanVec<V> ea, eh, mine = carry;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    ea.v[k] = L < 64 ? __shfl_up(A.v[k], L % 64, WAVE) : 1.0f;
+    eh.v[k] = L < 64 ? __shfl_up(H.v[k], L % 64, WAVE) : 0.0f;
+    if (run == 0) {
+      ea.v[k] = 1.0f;
+      eh.v[k] = 0.0f;
+    }
+  }
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      if (w == wave) mine.v[k] = carry.v[k];
+      carry.v[k] = fmaf(totals[w][0][l * V + k], carry.v[k], totals[w][1][l * V + k]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < V; ++k) mine.v[k] = fmaf(ea.v[k], mine.v[k], eh.v[k]);
+  return mine;
+}
+
+template <int V>
+__device__ __forceinline__ void scan_identity(ScanVec<V>& A, ScanVec<V>& H) {
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    A.v[k] = 1.0f;
+    H.v[k] = 0.0f;
+  }
+}
+
+// The pair of every chunk but the last: blockIdx.y = chunk.  A run of consecutive steps to each group of L threads.
+template <bool GRAD, int MODE, int V, int L, int R, int NT>
+__global__ __launch_bounds__(NT) void scan_totals_kernel(ScanArgs a, ScanSplit s) {
+  constexpr int NW = NT / 64, RUNS = NT / L;
+  __shared__ __attribute__((aligned(16))) float totals[NW][2][L * V];
+  const ScanPlace<V, L> p(a, s, blockIdx.y);
+  const unsigned run = threadIdx.x / L;
+  const size_t per = ((p.u1 - p.u0 + RUNS - 1) / RUNS + R - 1) / R * R;
+  const size_t begin = p.u0 + run * per, end = begin + per < p.u1 ? begin + per : p.u1;
+  ScanVec<V> A, H;
+  scan_identity(A, H);
+  for (size_t u = begin; u < end; u += R) {
+    ScanVec<V> g[R], x[R];
+    scan_load_rows<GRAD, V, R>(g, a.gate, a, p.b, p.c, p.nv, u, end);
+    scan_load_rows<GRAD, V, R>(x, GRAD ? a.dh : a.x, a, p.b, p.c, p.nv, u, end);
+    scan_fold<GRAD, MODE, V, R>(g, x, u, end, g, x, A, H);
+  }
+  scan_join_wave<V, L>(A, H, totals);
+  __syncthreads();
+  if (threadIdx.x >= L) return;
+  scan_identity(A, H);
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
+      H.v[k] = fmaf(totals[w][0][threadIdx.x * V + k], H.v[k], totals[w][1][threadIdx.x * V + k]);
+      A.v[k] *= totals[w][0][threadIdx.x * V + k];
+    }
+  }
+  float* o = s.pairs + ((size_t)blockIdx.y * a.batch + p.b) * 2 * a.channels + p.c;
+#pragma unroll
+  for (int k = 0; k < V; ++k)
+    if (k < p.nv) {
+      o[k] = A.v[k];
+      o[a.channels + k] = H.v[k];
+      if (!GRAD && blockIdx.y == 0 && a.h0) s.h0[p.b * a.channels + p.c + k] = a.h0[p.b * a.channels + p.c + k];
+    }
+}
+
+template <bool GRAD, int MODE, int V, int L, int R, int NT>
+__global__ __launch_bounds__(NT) void scan_tile_kernel(ScanArgs a, ScanSplit s) {
+  constexpr int NW = NT / 64, TILE = NT / L * R;
+  __shared__ __attribute__((aligned(16))) float totals[2][NW][2][L * V];  // two tiles' in turn: one barrier a tile
+  const ScanPlace<V, L> p(a, s, blockIdx.y);
+  const unsigned run = threadIdx.x / L;
+  const size_t state = p.b * a.channels + p.c;
+  ScanVec<V> carry, A, H;
+  scan_identity(A, carry);
+  const float* from = GRAD ? a.dh_last : gridDim.y > 1 && a.h0 ? s.h0 : a.h0;
+  if (from) carry = scan_load<V>(from + state, p.nv, 0.0f);
+  int buf = 0;
+  if (blockIdx.y > 0) {
+    // the chunks before this one: a run of consecutive chunks to each group of L threads
+    const unsigned before = blockIdx.y, per = (before + NT / L - 1) / (NT / L);
+    const unsigned q0 = run * per, q1 = q0 + per < before ? q0 + per : before;
+    scan_identity(A, H);
+    for (unsigned q = q0; q < q1; ++q) {
+      const float* o = s.pairs + ((size_t)q * a.batch + p.b) * 2 * a.channels + p.c;
+      const ScanVec<V> pa = scan_load<V>(o, p.nv, 1.0f), ph = scan_load<V>(o + a.channels, p.nv, 0.0f);
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        H.v[k] = fmaf(pa.v[k], H.v[k], ph.v[k]);
+        A.v[k] *= pa.v[k];
+      }
+    }
+    scan_join_wave<V, L>(A, H, totals[0]);
+    __syncthreads();
+    scan_reach<V, L, NW>(A, H, carry, totals[0]);
+    buf = 1;
+  }
+  ScanRun<GRAD, MODE, V, R> next;
+  scan_load_run<GRAD, MODE, V, R>(next, a, p.b, p.c, p.nv, p.u0 + run * R, p.u1);
+  for (size_t base = p.u0; base < p.u1; base += TILE, buf ^= 1) {
+    ScanRun<GRAD, MODE, V, R> now = next;
+    const size_t u = base + run * R;
+    if (base + TILE < p.u1) scan_load_run<GRAD, MODE, V, R>(next, a, p.b, p.c, p.nv, u + TILE, p.u1);
+    ScanVec<V> co[R], in[R];
+    scan_identity(A, H);
+    scan_fold<GRAD, MODE, V, R>(now.g, GRAD ? now.dh : now.x, u, p.u1, co, in, A, H);
+    scan_join_wave<V, L>(A, H, totals[buf]);
+    __syncthreads();
+    ScanVec<V> h = scan_reach<V, L, NW>(A, H, carry, totals[buf]);
+    if (p.nv == 0) continue;
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      if (u + r >= p.u1) break;
+      const size_t at = (p.b * a.steps + (GRAD ? a.steps - 1 - (u + r) : u + r)) * a.channels + p.c;
+      if (!GRAD) {
+#pragma unroll
+        for (int k = 0; k < V; ++k) h.v[k] = fmaf(co[r].v[k], h.v[k], in[r].v[k]);
+        scan_store<V>(a.h_out + at, h, p.nv);
+        if (u + r == a.steps - 1 && a.h_last) scan_store<V>(a.h_last + state, h, p.nv);
+        continue;
+      }
+      ScanVec<V> dg, dx;
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float d = now.dh[GRAD ? r : 0].v[k] + h.v[k], before = now.before[GRAD ? r : 0].v[k];
+        h.v[k] = co[r].v[k] * d;
+        if (MODE == SLHIP_SCAN_LINEAR) {
+          dg.v[k] = d * before;
+          dx.v[k] = d;
+        } else {
+          dx.v[k] = d * in[r].v[k];
+          dg.v[k] = (dx.v[k] * co[r].v[k]) * (before - now.x[GRAD && MODE == SLHIP_SCAN_LINEAR ? 0 : r].v[k]);
+        }
+      }
+      if (a.dgate) scan_grad_store<V>(a.dgate + at, dg, p.nv, a.beta);
+      if (a.dx) scan_grad_store<V>(a.dx + at, dx, p.nv, a.beta);
+      if (u + r == a.steps - 1 && a.dh0) scan_grad_store<V>(a.dh0 + state, h, p.nv, a.beta);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- host side
+template <bool GRAD, int MODE, int V, int L, int R>
+static int32_t scan_launch_tiles(slhip_ctx* ctx, const ScanArgs& a) {
+  constexpr int NT = 256, TILE = NT / L * R;
+  const size_t groups = a.batch * ((a.channels + L * V - 1) / (L * V));
+  if (groups > MAX_GRID) {
+    set_error("slhip_gated_scan: too many channels for one launch");
+    return SLHIP_EINVAL;
+  }
+  ScanSplit s = {a.steps, nullptr, nullptr};
+  size_t chunks = 1;
+  const size_t state = a.batch * a.channels;
+  if (groups < (size_t)ctx->num_cu) {
+    chunks = ((size_t)ctx->num_cu * 2 + groups - 1) / groups;
+    const size_t most = a.steps / (4 * TILE);
+    if (chunks > most) chunks = most;
+    const size_t room = ctx->workspace_bytes / (state * sizeof(float));  // states that the workspace holds
+    if (chunks > 1 && 2 * (chunks - 1) + 1 > room) chunks = room > 2 ? (room - 1) / 2 + 1 : 1;
+    if (chunks < 1) chunks = 1;
+  }
+  if (chunks > 1) {
+    s.chunk = ((a.steps + chunks - 1) / chunks + TILE - 1) / TILE * TILE;
+    chunks = (a.steps + s.chunk - 1) / s.chunk;
+  }
+  if (chunks > 1) {
+    s.h0 = (float*)ctx->workspace;
+    s.pairs = s.h0 + state;
+    hipLaunchKernelGGL((scan_totals_kernel<GRAD, MODE, V, L, R, NT>), dim3((unsigned)groups, (unsigned)(chunks - 1)), dim3(NT), 0, ctx->stream,
+                       a, s);
+    const int32_t rc = post_launch();
+    if (rc) return rc;
+  }
+  hipLaunchKernelGGL((scan_tile_kernel<GRAD, MODE, V, L, R, NT>), dim3((unsigned)groups, (unsigned)chunks), dim3(NT), 0, ctx->stream, a, s);
+  return post_launch();
 }
 
 template <bool GRAD, int MODE>
 static int32_t scan_launch(slhip_ctx* ctx, const ScanArgs& a) {
+  if (a.steps > 8) {
+    if (a.channels > 16) return scan_launch_tiles<GRAD, MODE, 4, 8, 4>(ctx, a);
+    if (a.channels > 8) return scan_launch_tiles<GRAD, MODE, 4, 4, 4>(ctx, a);
+    if (a.channels > 3) return scan_launch_tiles<GRAD, MODE, 4, 2, 4>(ctx, a);
+    if (a.channels > 1) return scan_launch_tiles<GRAD, MODE, 1, 4, 8>(ctx, a);
+    return scan_launch_tiles<GRAD, MODE, 1, 1, 8>(ctx, a);
+  }
   const int V = a.channels >= 4 ? 4 : 1;
   const size_t threads = a.batch * ((a.channels + V - 1) / V);
   if (!grid_fits(threads, 256)) {
