@@ -193,6 +193,24 @@ __device__ __forceinline__ void st4s(float* p, float4 v) {
 __device__ __forceinline__ float ld1s(const float* p) { return __builtin_nontemporal_load(p); }
 __device__ __forceinline__ void st1s(float* p, float v) { __builtin_nontemporal_store(v, p); }
 
+// 1/(1 + exp(-z)) and 1/(1 + exp(z)), which add up to one, each to about two units in its last place at either end: with
+// e = exp(-|z|) nothing overflows, and the smaller of the two is e / (1 + e), not a difference.  The hardware's 2^x and
+// reciprocal with a correction each (the rounding of |z| log2(e) is put back as a factor 1 + lo ln 2; one Newton step),
+// since the library's exponential and the IEEE quotient take twice the instructions: the gated recurrence, where the
+// sigmoid is most of the arithmetic, is bound by it.
+__device__ __forceinline__ void sigmoid_pair(float z, float& s, float& rest) {
+  float t = fabsf(z);
+  t = t > 150.0f ? 150.0f : t;  // keeps NaN; e is zero from 104 on
+  const float hi = -t * 1.44269502162933349609375f;                                   // log2(e), rounded
+  const float lo = fmaf(-t, 1.925963033500011079e-8f, fmaf(-t, 1.44269502162933349609375f, -hi));  // and what that left
+  const float e0 = __builtin_amdgcn_exp2f(hi);
+  const float e = fmaf(e0, lo * 0.693147180559945309f, e0);
+  const float d = 1.0f + e, r0 = __builtin_amdgcn_rcpf(d);
+  const float big = fmaf(fmaf(-d, r0, 1.0f), r0, r0), small = e * big;
+  s = z >= 0.0f ? big : small;
+  rest = z >= 0.0f ? small : big;
+}
+
 // d f(l, r) / d l   and   d f(l, r) / d r, as the reference's tests write them
 // (src/ops2/col_op/grad/cpu.rs:115,146: 1/rhs and lhs / -(rhs*rhs) for div)
 __device__ __forceinline__ float bc_dl(int op, float /*l*/, float r) {
