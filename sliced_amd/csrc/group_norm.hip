@@ -5,11 +5,24 @@
 //   g = dout * act'(u), gx = g * weight, < > the mean over the group:
 //   dx = rstd * (gx - <gx> - hat * <gx * hat>)       dweight = sum g * hat       dbias = sum g
 //
-// HBM is the bound: 8 bytes an element forward, 12 backward, if x (and dout) are read once.
+// HBM is the bound: 8 bytes an element forward, 12 backward, if x (and dout) are read once.  Three families of kernels:
 //
-// A workgroup works on one group of one sample: a thread keeps to one vector of V channels of the group
-// and steps through the positions, so that weights, biases and the per-channel sums of the backward pass
-// stay in its registers.  V is the widest of 4, 2, 1 that divides the group's channels.
+//   rows     one position a sample (a norm of every row): a row of a group's channels lives in the registers of 4 to 64
+//            lanes or of a workgroup, which go on to further rows of the same group with its weights - and, backward,
+//            the sums for their gradients - in registers;
+//   on chip  all positions of a window of groups fit the registers of a workgroup: x (and dout) are read once;
+//   two pass larger ones: a kernel that takes sums, one that applies them.  Runs of positions of a sample go to workgroups
+//            of their own, and the second kernel starts where the first one ended, with what the last-level cache still
+//            holds.
+//
+// In the latter two a window is a run of whole groups, about 64 vectors of channels wide (1 KiB of a row of x): narrower
+// pieces of rows than that cost HBM bandwidth.  Groups wider than a workgroup are cut.  A thread keeps to one vector of V
+// channels and steps through the positions, so that weights, biases and per-channel sums stay in registers.  V is the
+// widest of 4, 2, 1 that divides a group's channels.
+#include <initializer_list>
+#include <type_traits>
+#include <utility>
+
 #include "common.hpp"
 
 namespace slhip {
@@ -17,7 +30,9 @@ namespace slhip {
 struct NormArgs {
   size_t N, P, C, G, cg;  // samples, positions, channels, groups, channels of a group
   size_t n0;              // first sample of this launch
-  unsigned wv, windows;   // vectors of a group's channels that a workgroup covers; such windows of a group
+  unsigned lanes;         // vectors of channels that a workgroup covers
+  unsigned together;      // groups of a window, or 1 where a group is cut into
+  unsigned windows;       //   this many windows
   unsigned rows;          // positions that a workgroup takes at a time
   unsigned chunks;        // runs of positions of a sample, a workgroup each
   size_t chunk;           // positions of a run
@@ -33,7 +48,7 @@ struct NormArgs {
   float* dx;
   float beta;
   float* part;            // workspace: two floats for every group and workgroup of it
-  float* cols;            // workspace: [samples * chunks][2][channels]
+  float* cols;            // workspace: [samples * chunks][2][channels], dweight's and dbias's terms
 };
 
 template <int V>
@@ -78,7 +93,11 @@ __device__ __forceinline__ NormVec<V> norm_param(const float* p, size_t c, float
 template <int ACT>
 __device__ __forceinline__ float norm_act(float u) {
   if (ACT == SLHIP_ACT_RELU) return (u >= 0.0f ? 1.0f : 0.0f) * u;
-  if (ACT == SLHIP_ACT_SILU) return u / (1.0f + expf(-u));
+  if (ACT == SLHIP_ACT_SILU) {
+    float q, rest;
+    sigmoid_pair(u, q, rest);
+    return u * q;
+  }
   if (ACT == SLHIP_ACT_GELU) return 0.5f * u * (1.0f + erff(u * 0.70710678118654752f));
   return u;
 }
@@ -86,44 +105,75 @@ template <int ACT>
 __device__ __forceinline__ float norm_act_grad(float u) {
   if (ACT == SLHIP_ACT_RELU) return u >= 0.0f ? 1.0f : 0.0f;
   if (ACT == SLHIP_ACT_SILU) {
-    const float q = 1.0f / (1.0f + expf(-u));
-    return q * (1.0f + u * (1.0f - q));
+    float q, rest;
+    sigmoid_pair(u, q, rest);
+    return q * (1.0f + u * rest);
   }
   if (ACT == SLHIP_ACT_GELU)
     return 0.5f * (1.0f + erff(u * 0.70710678118654752f)) + u * expf(-0.5f * u * u) * 0.39894228040143268f;
   return 1.0f;
 }
+// One element of either direction.
+template <int ACT>
+__device__ __forceinline__ float norm_out(float x, float mean, float rstd, float w, float b) {
+  return norm_act<ACT>(((x - mean) * rstd) * w + b);
+}
+template <int ACT>
+__device__ __forceinline__ float norm_upstream(float x, float g, float mean, float rstd, float w, float b, float& hat) {
+  hat = (x - mean) * rstd;
+  return g * norm_act_grad<ACT>(hat * w + b);
+}
 
-// Where a workgroup works.  Its number walks the groups fastest, and numbers are dealt out so that an XCD gets a
-// contiguous run of them: the 128-byte lines that neighbouring groups share then meet in one L2.
+// Where a workgroup works.  Its number walks the windows fastest, and numbers are dealt out so that an XCD gets a contiguous
+// run of them: the 128-byte lines that neighbouring windows share then meet in one L2.
 struct NormPlace {
-  bool some;        // the workgroup has work
-  size_t n, g;      // sample, group
-  unsigned part;    // of the group: window and run of positions
-  size_t c;         // this thread's first channel
+  bool some;          // the workgroup has work
+  size_t n, g;        // sample, this thread's group
+  unsigned part;      // of the group: window and run of positions
+  unsigned local;     // this thread's group within the window
+  size_t c;           // its first channel
   size_t first, end;  // its first position, and the end of the workgroup's run
-  unsigned row;     // its place among the positions taken at a time
+  unsigned lane, row; // its place in the window and among the positions taken at a time
   bool active;
 };
-template <int V>
-__device__ __forceinline__ NormPlace norm_place(const NormArgs& a) {
+template <int V, int NT>
+__device__ __forceinline__ NormPlace norm_place(const NormArgs& a, bool backwards) {
   NormPlace p;
   const size_t per = (a.blocks + 7) / 8;
   size_t id = (size_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
   p.some = (blockIdx.x >> 3) < per && id < a.blocks;
   if (!p.some) id = 0;
-  p.g = id % a.G;
-  id /= a.G;
-  const unsigned window = (unsigned)(id % a.windows);
-  id /= a.windows;
+  if (backwards) id = a.blocks - 1 - id;
+  const unsigned cgv = (unsigned)(a.cg / V);
+  const size_t across = (a.G + a.together - 1) / a.together;
+  p.lane = threadIdx.x % a.lanes;
+  p.row = threadIdx.x / a.lanes;
+  const size_t window = id % (across * a.windows);
+  id /= across * a.windows;
   const unsigned chunk = (unsigned)(id % a.chunks);
   p.n = a.n0 + id / a.chunks;
-  p.part = chunk * a.windows + window;
-  const unsigned cgv = (unsigned)(a.cg / V), lane = threadIdx.x % a.wv;
-  const unsigned v = window * a.wv + lane;
-  p.row = threadIdx.x / a.wv;
-  p.active = p.some && p.row < a.rows && v < cgv;
-  p.c = p.g * a.cg + (size_t)(v < cgv ? v : 0) * V;
+  p.active = p.some && p.row < a.rows;
+  size_t v;
+  if (a.windows > 1) {
+    const unsigned piece = (unsigned)(window % a.windows);
+    p.g = window / a.windows;
+    p.local = 0;
+    p.part = chunk * a.windows + piece;
+    v = (size_t)piece * a.lanes + p.lane;
+    p.active = p.active && v < cgv;
+    v = p.g * cgv + (v < cgv ? v : 0);
+  } else {
+    p.local = p.lane / cgv;
+    p.g = window * a.together + p.local;
+    p.part = chunk;
+    p.active = p.active && p.g < a.G;
+    v = window * a.lanes + p.lane;
+    if (p.g >= a.G) {
+      p.g = a.G - 1;
+      v = 0;
+    }
+  }
+  p.c = v * V;
   const size_t begin = (size_t)chunk * a.chunk;
   p.end = begin + a.chunk < a.P ? begin + a.chunk : a.P;
   p.first = begin + p.row;
@@ -131,43 +181,99 @@ __device__ __forceinline__ NormPlace norm_place(const NormArgs& a) {
   return p;
 }
 
-// Values of a workgroup's part of its group.
+// Values of a part of a group.
 template <int V>
 __device__ __forceinline__ float norm_count(const NormArgs& a, unsigned part) {
-  const unsigned window = part % a.windows, chunk = part / a.windows;
+  const unsigned piece = part % a.windows, chunk = part / a.windows;
   const size_t begin = (size_t)chunk * a.chunk, end = begin + a.chunk < a.P ? begin + a.chunk : a.P;
-  const size_t cgv = a.cg / V, v0 = (size_t)window * a.wv, v1 = v0 + a.wv < cgv ? v0 + a.wv : cgv;
+  const size_t cgv = a.cg / V, v0 = (size_t)piece * a.lanes, v1 = a.windows > 1 && v0 + a.lanes < cgv ? v0 + a.lanes : cgv;
   return (float)((end - begin) * (v1 - v0) * V);
 }
 
-// Mean and sum of squared differences from it of one workgroup's part.  A thread sums differences from the first
-// value it meets, and threads and parts are then joined by their means: a group far from zero keeps its variance.
+// Sums of two values over the threads of each group of the window: a wave takes the threads of one group at a time, in a
+// fixed order.  Threads without work bring zeros.
+template <int NT>
+struct NormSums {
+  float2 value[NT];
+  float2 total[64];
+};
+template <int V, int NT>
+__device__ __forceinline__ float2 norm_group_sums(const NormArgs& a, const NormPlace& p, float x, float y, NormSums<NT>& s) {
+  const unsigned cgv = a.windows > 1 ? a.lanes : (unsigned)(a.cg / V), lane = threadIdx.x & 63;
+  __syncthreads();  // the totals of an earlier call have been read
+  s.value[threadIdx.x] = p.active ? make_float2(x, y) : make_float2(0.0f, 0.0f);
+  __syncthreads();
+  for (unsigned k = threadIdx.x >> 6; k < a.together; k += NT / 64) {
+    float2 t = make_float2(0.0f, 0.0f);
+    for (unsigned i = lane; i < a.rows * cgv; i += 64) {
+      const unsigned r = i / cgv;
+      const float2 v = s.value[r * a.lanes + k * cgv + (i - r * cgv)];
+      t.x += v.x;
+      t.y += v.y;
+    }
+    t.x = wave_reduce<SumOp>(t.x);
+    t.y = wave_reduce<SumOp>(t.y);
+    if (lane == 0) s.total[k] = t;
+  }
+  __syncthreads();
+  return s.total[p.local];
+}
+
+// A working thread's place among those of its group in the workgroup.
+struct NormTeam {
+  unsigned rank, size;
+};
+template <int V>
+__device__ __forceinline__ NormTeam norm_team(const NormArgs& a, const NormPlace& p) {
+  const unsigned cgv = (unsigned)(a.cg / V);
+  // a piece of a group: the lanes that this window really has
+  const unsigned piece = a.windows > 1 ? p.part % a.windows : 0;
+  const unsigned mine = a.windows > 1 ? (cgv - piece * a.lanes < a.lanes ? cgv - piece * a.lanes : a.lanes) : cgv;
+  const unsigned lane = a.windows > 1 ? p.lane : p.lane - p.local * cgv;
+  return NormTeam{p.row * mine + lane, a.rows * mine};
+}
+
+// A thread's sums over its positions, 4 of them requested at a time.
+template <int V, class F>
+__device__ __forceinline__ void norm_each(const NormArgs& a, const NormPlace& p, F&& f) {
+  const size_t step = (size_t)a.rows * a.C;
+  size_t at = (p.n * a.P + p.first) * a.C + p.c, r = p.first;
+  for (; r + 3 * (size_t)a.rows < p.end; r += 4 * (size_t)a.rows, at += 4 * step) f(at, step, std::integral_constant<int, 4>());
+  for (; r < p.end; r += a.rows, at += step) f(at, step, std::integral_constant<int, 1>());
+}
+
+// ---------------------------------------------------------------- two pass
+// Mean and sum of squared differences from it of one workgroup's part of each of its groups.  A thread sums differences from
+// the first value it meets, and threads and parts are then joined by their means: a group far from zero keeps its variance.
 template <int V>
 __global__ __launch_bounds__(256) void norm_stats_kernel(NormArgs a) {
-  __shared__ float red[4];
-  const NormPlace p = norm_place<V>(a);
+  __shared__ NormSums<256> sums;
+  const NormPlace p = norm_place<V, 256>(a, false);
   if (!p.some) return;
-  float s1 = 0.0f, s2 = 0.0f, shift = 0.0f, count = 0.0f;
-  const float* at = a.x + (p.n * a.P + p.first) * a.C + p.c;
-  if (p.first < p.end) shift = at[0];
-#pragma unroll 4
-  for (size_t r = p.first; r < p.end; r += a.rows, at += a.rows * a.C) {
-    const NormVec<V> v = norm_load<V>(at);
+  float s1 = 0.0f, s2 = 0.0f, count = 0.0f;
+  const float shift = a.x[(p.n * a.P + (p.first < p.end ? p.first : 0)) * a.C + p.c];
+  norm_each<V>(a, p, [&](size_t at, size_t step, auto some) {
+    constexpr int U = decltype(some)::value;
+    NormVec<V> v[U];
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const float d = v.v[k] - shift;
-      s1 += d;
-      s2 = fmaf(d, d, s2);
-    }
-    count += (float)V;
-  }
+    for (int i = 0; i < U; ++i) v[i] = norm_load<V>(a.x + at + i * step);
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float d = v[i].v[k] - shift;
+        s1 += d;
+        s2 = fmaf(d, d, s2);
+      }
+    count += (float)(U * V);
+  });
   const float m = count > 0.0f ? s1 / count : 0.0f;
-  const float here = shift + m;                       // the thread's mean
-  const float spread = fmaxf(s2 - s1 * m, 0.0f);      // and its sum of squared differences
-  const float mean = block_reduce<SumOp>(count * here, red) / norm_count<V>(a, p.part);
+  const float here = shift + m;                   // the thread's mean
+  const float spread = fmaxf(s2 - s1 * m, 0.0f);  // and its sum of squared differences
+  const float mean = norm_group_sums<V, 256>(a, p, count * here, 0.0f, sums).x / norm_count<V>(a, p.part);
   const float away = here - mean;
-  const float m2 = block_reduce<SumOp>(spread + count * (away * away), red);
-  if (threadIdx.x == 0) {
+  const float m2 = norm_group_sums<V, 256>(a, p, spread + count * (away * away), 0.0f, sums).x;
+  if (p.active && norm_team<V>(a, p).rank == 0) {
     float* o = a.part + 2 * (((p.n - a.n0) * a.G + p.g) * (a.chunks * a.windows) + p.part);
     o[0] = mean;
     o[1] = m2;
@@ -176,63 +282,48 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormArgs a) {
 
 template <int V, int ACT>
 __global__ __launch_bounds__(256) void norm_apply_kernel(NormArgs a) {
-  __shared__ float red[4];
-  const NormPlace p = norm_place<V>(a);
+  __shared__ NormSums<256> sums;
+  const NormPlace p = norm_place<V, 256>(a, true);
   if (!p.some) return;
-  const size_t group = (p.n - a.n0) * a.G + p.g;
+  // the threads of a group join its parts
   const unsigned parts = a.chunks * a.windows;
-  const float* in = a.part + 2 * group * parts;
+  const float* in = a.part + 2 * ((p.n - a.n0) * a.G + p.g) * parts;
   const float total = (float)(a.P * a.cg);
+  const NormTeam t = norm_team<V>(a, p);
   float s = 0.0f;
-  for (unsigned i = threadIdx.x; i < parts; i += 256) s += norm_count<V>(a, i) * in[2 * i];
-  const float mean = block_reduce<SumOp>(s, red) / total;
+  for (unsigned i = t.rank; i < parts; i += t.size) s += norm_count<V>(a, i) * in[2 * i];
+  const float mean = norm_group_sums<V, 256>(a, p, s, 0.0f, sums).x / total;
   s = 0.0f;
-  for (unsigned i = threadIdx.x; i < parts; i += 256) {
+  for (unsigned i = t.rank; i < parts; i += t.size) {
     const float away = in[2 * i] - mean;
     s += in[2 * i + 1] + norm_count<V>(a, i) * (away * away);
   }
-  const float rstd = 1.0f / sqrtf(block_reduce<SumOp>(s, red) / total + a.eps);
-  if (p.part == 0 && threadIdx.x == 0) {
+  const float rstd = 1.0f / sqrtf(norm_group_sums<V, 256>(a, p, s, 0.0f, sums).x / total + a.eps);
+  if (!p.active) return;
+  if (p.part == 0 && t.rank == 0) {
     if (a.mean) a.mean[p.n * a.G + p.g] = mean;
     if (a.rstd) a.rstd[p.n * a.G + p.g] = rstd;
   }
-  if (!p.active) return;
   const NormVec<V> w = norm_param<V>(a.w, p.c, 1.0f), b = norm_param<V>(a.b, p.c, 0.0f);
-  size_t at = (p.n * a.P + p.first) * a.C + p.c;
-#pragma unroll 4
-  for (size_t r = p.first; r < p.end; r += a.rows, at += a.rows * a.C) {
-    NormVec<V> v = norm_load<V>(a.x + at);
+  norm_each<V>(a, p, [&](size_t at, size_t step, auto some) {
+    constexpr int U = decltype(some)::value;
+    NormVec<V> v[U];
 #pragma unroll
-    for (int k = 0; k < V; ++k) v.v[k] = norm_act<ACT>(((v.v[k] - mean) * rstd) * w.v[k] + b.v[k]);
-    norm_store<V>(a.out + at, v);
-  }
+    for (int i = 0; i < U; ++i) v[i] = norm_load<V>(a.x + at + i * step);
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[i].v[k] = norm_out<ACT>(v[i].v[k], mean, rstd, w.v[k], b.v[k]);
+      norm_store<V>(a.out + at + i * step, v[i]);
+    }
+  });
 }
 
-// Backward, first pass: per channel the sums of g and g * hat over the workgroup's positions, and over its channels
-// those weighted by the weights.
-template <int V, int ACT>
-__global__ __launch_bounds__(256) void norm_grad_sums_kernel(NormArgs a) {
-  __shared__ float red[4];
-  __shared__ float sums[256][2 * V + 1];  // (one word more a row: rows start on different banks)
-  const NormPlace p = norm_place<V>(a);
-  if (!p.some) return;
-  const float mean = a.mean[p.n * a.G + p.g], rstd = a.rstd[p.n * a.G + p.g];
-  const NormVec<V> w = norm_param<V>(a.w, p.c, 1.0f), b = norm_param<V>(a.b, p.c, 0.0f);
-  float s1[V], s2[V];
-#pragma unroll
-  for (int k = 0; k < V; ++k) s1[k] = s2[k] = 0.0f;
-  size_t at = (p.n * a.P + p.first) * a.C + p.c;
-#pragma unroll 4
-  for (size_t r = p.first; r < p.end; r += a.rows, at += a.rows * a.C) {
-    const NormVec<V> v = norm_load<V>(a.x + at), g = norm_load<V>(a.g + at);
-#pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const float hat = (v.v[k] - mean) * rstd;
-      const float gu = g.v[k] * norm_act_grad<ACT>(hat * w.v[k] + b.v[k]);
-      s1[k] += gu;
-      s2[k] = fmaf(gu, hat, s2[k]);
-    }
-  }
+// Sums over the positions that the workgroup's threads of one vector of channels took, left with those of row 0: a
+// tree over the rows.
+template <int V, int NT>
+__device__ __forceinline__ void norm_channel_sums(const NormArgs& a, const NormPlace& p, const float* s1, const float* s2,
+                                                  float (*sums)[2 * V + 1]) {
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     sums[threadIdx.x][2 * k] = s1[k];
@@ -244,69 +335,405 @@ __global__ __launch_bounds__(256) void norm_grad_sums_kernel(NormArgs a) {
     __syncthreads();
     if (p.row < half && p.row + half < a.rows) {
 #pragma unroll
-      for (int k = 0; k < 2 * V; ++k) sums[threadIdx.x][k] += sums[threadIdx.x + half * a.wv][k];
+      for (int k = 0; k < 2 * V; ++k) sums[threadIdx.x][k] += sums[threadIdx.x + half * a.lanes][k];
     }
   }
-  const bool mine = p.active && p.row == 0;  // (row 0 holds the totals, which its own threads added last)
-  float ga = 0.0f, gb = 0.0f;
-  if (mine) {
-    float* o = a.cols ? a.cols + (((p.n - a.n0) * a.chunks + p.part / a.windows) * 2) * a.C + p.c : nullptr;
+}
+template <int V>
+__device__ __forceinline__ void norm_put_columns(const NormArgs& a, const NormPlace& p, const float* sums, size_t row) {
+  float* o = a.cols + row * 2 * a.C + p.c;
 #pragma unroll
-    for (int k = 0; k < V; ++k) {
-      const float x = sums[threadIdx.x][2 * k], y = sums[threadIdx.x][2 * k + 1];
-      ga = fmaf(w.v[k], x, ga);
-      gb = fmaf(w.v[k], y, gb);
-      if (o) {
-        o[k] = y;
-        o[a.C + k] = x;
-      }
-    }
+  for (int k = 0; k < V; ++k) {
+    o[k] = sums[2 * k + 1];
+    o[a.C + k] = sums[2 * k];
   }
-  ga = block_reduce<SumOp>(ga, red);
-  gb = block_reduce<SumOp>(gb, red);
-  if (threadIdx.x == 0) {
+}
+
+// Backward, first pass: per channel the sums of g and g * hat over the workgroup's positions, and over a group's channels
+// those weighted by the weights.
+template <int V, int ACT>
+__global__ __launch_bounds__(256) void norm_grad_sums_kernel(NormArgs a) {
+  __shared__ NormSums<256> groups;
+  __shared__ float sums[256][2 * V + 1];  // (one word more a row: rows start on different banks)
+  const NormPlace p = norm_place<V, 256>(a, false);
+  if (!p.some) return;
+  const float mean = a.mean[p.n * a.G + p.g], rstd = a.rstd[p.n * a.G + p.g];
+  const NormVec<V> w = norm_param<V>(a.w, p.c, 1.0f), b = norm_param<V>(a.b, p.c, 0.0f);
+  float s1[V], s2[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) s1[k] = s2[k] = 0.0f;
+  norm_each<V>(a, p, [&](size_t at, size_t step, auto some) {
+    constexpr int U = decltype(some)::value;
+    NormVec<V> v[U], g[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      v[i] = norm_load<V>(a.x + at + i * step);
+      g[i] = norm_load<V>(a.g + at + i * step);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        float hat;
+        const float gu = norm_upstream<ACT>(v[i].v[k], g[i].v[k], mean, rstd, w.v[k], b.v[k], hat);
+        s1[k] += gu;
+        s2[k] = fmaf(gu, hat, s2[k]);
+      }
+  });
+  if (a.cols) {
+    norm_channel_sums<V, 256>(a, p, s1, s2, sums);
+    if (p.active && p.row == 0) norm_put_columns<V>(a, p, sums[threadIdx.x], (p.n - a.n0) * a.chunks + p.part / a.windows);
+  }
+  float ga = 0.0f, gb = 0.0f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    ga = fmaf(w.v[k], s1[k], ga);
+    gb = fmaf(w.v[k], s2[k], gb);
+  }
+  const float2 t = norm_group_sums<V, 256>(a, p, ga, gb, groups);
+  if (p.active && norm_team<V>(a, p).rank == 0) {
     float* o = a.part + 2 * (((p.n - a.n0) * a.G + p.g) * (a.chunks * a.windows) + p.part);
-    o[0] = ga;
-    o[1] = gb;
+    o[0] = t.x;
+    o[1] = t.y;
   }
 }
 
 template <int V, int ACT>
 __global__ __launch_bounds__(256) void norm_grad_apply_kernel(NormArgs a) {
-  __shared__ float red[4];
-  const NormPlace p = norm_place<V>(a);
+  __shared__ NormSums<256> sums;
+  const NormPlace p = norm_place<V, 256>(a, true);
   if (!p.some) return;
   const float mean = a.mean[p.n * a.G + p.g], rstd = a.rstd[p.n * a.G + p.g];
   const unsigned parts = a.chunks * a.windows;
   const float* in = a.part + 2 * ((p.n - a.n0) * a.G + p.g) * parts;
   const float total = (float)(a.P * a.cg);
   float ga = 0.0f, gb = 0.0f;
-  for (unsigned i = threadIdx.x; i < parts; i += 256) {
+  const NormTeam t = norm_team<V>(a, p);
+  for (unsigned i = t.rank; i < parts; i += t.size) {
     ga += in[2 * i];
     gb += in[2 * i + 1];
   }
-  ga = block_reduce<SumOp>(ga, red) / total;
-  gb = block_reduce<SumOp>(gb, red) / total;
+  const float2 both = norm_group_sums<V, 256>(a, p, ga, gb, sums);
   if (!p.active) return;
+  ga = both.x / total;
+  gb = both.y / total;
   const NormVec<V> w = norm_param<V>(a.w, p.c, 1.0f), b = norm_param<V>(a.b, p.c, 0.0f);
-  size_t at = (p.n * a.P + p.first) * a.C + p.c;
-#pragma unroll 4
-  for (size_t r = p.first; r < p.end; r += a.rows, at += a.rows * a.C) {
-    const NormVec<V> v = norm_load<V>(a.x + at), g = norm_load<V>(a.g + at);
-    NormVec<V> d;
+  norm_each<V>(a, p, [&](size_t at, size_t step, auto some) {
+    constexpr int U = decltype(some)::value;
+    NormVec<V> v[U], g[U];
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+      v[i] = norm_load<V>(a.x + at + i * step);
+      g[i] = norm_load<V>(a.g + at + i * step);
+    }
+#pragma unroll
+    for (int i = 0; i < U; ++i) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        float hat;
+        const float gx = norm_upstream<ACT>(v[i].v[k], g[i].v[k], mean, rstd, w.v[k], b.v[k], hat) * w.v[k];
+        v[i].v[k] = rstd * (gx - ga - hat * gb);
+      }
+      if (a.beta != 0.0f) {
+        const NormVec<V> old = norm_load<V>(a.dx + at + i * step);
+#pragma unroll
+        for (int k = 0; k < V; ++k) v[i].v[k] = a.beta * old.v[k] + v[i].v[k];
+      }
+      norm_store<V>(a.dx + at + i * step, v[i]);
+    }
+  });
+}
+
+// ---------------------------------------------------------------- on chip
+// All P <= rows * K positions of a window in the registers of one workgroup: the variance from differences to the mean
+// itself, x read once.
+template <int V, int ACT, int NT, int K>
+__global__ __launch_bounds__(NT) void norm_chip_kernel(NormArgs a) {
+  __shared__ NormSums<NT> sums;
+  const NormPlace p = norm_place<V, NT>(a, false);
+  if (!p.some) return;
+  const size_t base = p.n * a.P * a.C + p.c;
+  NormVec<V> v[K];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {  // (positions past the end: the last one's values, left out below)
+    const size_t r = p.row + (size_t)i * a.rows;
+    v[i] = norm_load<V>(a.x + base + (r < a.P ? r : a.P - 1) * a.C);
+  }
+  const float total = (float)(a.P * a.cg);
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    float t = 0.0f;
+#pragma unroll
+    for (int k = 0; k < V; ++k) t += v[i].v[k];
+    s += p.row + (size_t)i * a.rows < a.P ? t : 0.0f;
+  }
+  const float mean = norm_group_sums<V, NT>(a, p, s, 0.0f, sums).x / total;
+  s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    float t = 0.0f;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const float hat = (v.v[k] - mean) * rstd;
-      const float gx = g.v[k] * norm_act_grad<ACT>(hat * w.v[k] + b.v[k]) * w.v[k];
-      d.v[k] = rstd * (gx - ga - hat * gb);
+      const float d = v[i].v[k] - mean;
+      t = fmaf(d, d, t);
     }
+    s += p.row + (size_t)i * a.rows < a.P ? t : 0.0f;
+  }
+  const float rstd = 1.0f / sqrtf(norm_group_sums<V, NT>(a, p, s, 0.0f, sums).x / total + a.eps);
+  if (!p.active) return;
+  if (norm_team<V>(a, p).rank == 0) {
+    if (a.mean) a.mean[p.n * a.G + p.g] = mean;
+    if (a.rstd) a.rstd[p.n * a.G + p.g] = rstd;
+  }
+  const NormVec<V> w = norm_param<V>(a.w, p.c, 1.0f), b = norm_param<V>(a.b, p.c, 0.0f);
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const size_t r = p.row + (size_t)i * a.rows;
+    if (r >= a.P) break;
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[i].v[k] = norm_out<ACT>(v[i].v[k], mean, rstd, w.v[k], b.v[k]);
+    norm_store<V>(a.out + base + r * a.C, v[i]);
+  }
+}
+
+template <int V, int ACT, int NT, int K>
+__global__ __launch_bounds__(NT) void norm_chip_grad_kernel(NormArgs a) {
+  __shared__ NormSums<NT> groups;
+  __shared__ float sums[NT][2 * V + 1];
+  const NormPlace p = norm_place<V, NT>(a, false);
+  if (!p.some) return;
+  const size_t base = p.n * a.P * a.C + p.c;
+  NormVec<V> v[K], g[K];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const size_t r = p.row + (size_t)i * a.rows, at = base + (r < a.P ? r : a.P - 1) * a.C;
+    v[i] = norm_load<V>(a.x + at);
+    g[i] = norm_load<V>(a.g + at);
+  }
+  const float mean = a.mean[p.n * a.G + p.g], rstd = a.rstd[p.n * a.G + p.g], total = (float)(a.P * a.cg);
+  const NormVec<V> w = norm_param<V>(a.w, p.c, 1.0f), b = norm_param<V>(a.b, p.c, 0.0f);
+  float s1[V], s2[V];
+#pragma unroll
+  for (int k = 0; k < V; ++k) s1[k] = s2[k] = 0.0f;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const bool in = p.row + (size_t)i * a.rows < a.P;
+#pragma unroll
+    for (int k = 0; k < V; ++k) {  // x becomes hat, dout becomes g
+      float hat;
+      const float gu = norm_upstream<ACT>(v[i].v[k], g[i].v[k], mean, rstd, w.v[k], b.v[k], hat);
+      v[i].v[k] = hat;
+      g[i].v[k] = gu;
+      s1[k] += in ? gu : 0.0f;
+      s2[k] = in ? fmaf(gu, hat, s2[k]) : s2[k];
+    }
+  }
+  if (a.cols) {
+    norm_channel_sums<V, NT>(a, p, s1, s2, sums);
+    if (p.active && p.row == 0) norm_put_columns<V>(a, p, sums[threadIdx.x], p.n - a.n0);
+  }
+  if (!a.dx) return;
+  float ga = 0.0f, gb = 0.0f;
+#pragma unroll
+  for (int k = 0; k < V; ++k) {
+    ga = fmaf(w.v[k], s1[k], ga);
+    gb = fmaf(w.v[k], s2[k], gb);
+  }
+  const float2 t = norm_group_sums<V, NT>(a, p, ga, gb, groups);
+  if (!p.active) return;
+  ga = t.x / total;
+  gb = t.y / total;
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const size_t r = p.row + (size_t)i * a.rows;
+    if (r >= a.P) break;
+    NormVec<V> d;
+#pragma unroll
+    for (int k = 0; k < V; ++k) d.v[k] = rstd * (g[i].v[k] * w.v[k] - ga - v[i].v[k] * gb);
     if (a.beta != 0.0f) {
-      const NormVec<V> old = norm_load<V>(a.dx + at);
+      const NormVec<V> old = norm_load<V>(a.dx + base + r * a.C);
 #pragma unroll
       for (int k = 0; k < V; ++k) d.v[k] = a.beta * old.v[k] + d.v[k];
     }
-    norm_store<V>(a.dx + at, d);
+    norm_store<V>(a.dx + base + r * a.C, d);
   }
+}
+
+// ---------------------------------------------------------------- rows
+// One position a sample: samples * groups rows of cg channels, one after the other in memory.  A team of threads - `lanes`
+// of a wave (BLOCK false), or the whole workgroup - holds a row, K vectors to a thread, and goes on to the row `teams`
+// further: teams is a multiple of the groups, so its group, and with it weights, biases and the columns of their
+// gradients, stays the same.
+struct NormRows {
+  unsigned lanes;
+  size_t teams;
+};
+
+template <bool BLOCK, int NT>
+__device__ __forceinline__ float2 norm_row_sums(float x, float y, unsigned lanes, float2* wave_sums) {
+  if (!BLOCK) {
+    for (unsigned o = lanes / 2; o > 0; o /= 2) {
+      x += __shfl_xor(x, o, WAVE);
+      y += __shfl_xor(y, o, WAVE);
+    }
+    return make_float2(x, y);
+  }
+  x = wave_reduce<SumOp>(x);
+  y = wave_reduce<SumOp>(y);
+  __syncthreads();  // the sums of an earlier call have been read
+  if ((threadIdx.x & 63) == 0) wave_sums[threadIdx.x >> 6] = make_float2(x, y);
+  __syncthreads();
+  float2 t = wave_sums[0];
+#pragma unroll
+  for (int i = 1; i < NT / 64; ++i) {
+    t.x += wave_sums[i].x;
+    t.y += wave_sums[i].y;
+  }
+  return t;
+}
+
+template <int V, int ACT, int NT, int K, bool BLOCK>
+__global__ __launch_bounds__(NT) void norm_rows_kernel(NormArgs a, NormRows t) {
+  __shared__ float2 wave_sums[NT / 64];
+  const unsigned lanes = BLOCK ? NT : t.lanes, lane = threadIdx.x % lanes, cgv = (unsigned)(a.cg / V);
+  const size_t team = (size_t)blockIdx.x * (NT / lanes) + threadIdx.x / lanes, rows = a.N * a.G;
+  if (team >= t.teams) return;
+  const size_t group = team % a.G;
+  size_t at[K];  // of a vector within the row; one past the end stands at the last and is left out
+  bool in[K];
+  NormVec<V> w[K], b[K];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const unsigned q = lane + i * lanes;
+    in[i] = q < cgv;
+    at[i] = (size_t)(in[i] ? q : cgv - 1) * V;
+    w[i] = norm_param<V>(a.w, group * a.cg + at[i], 1.0f);
+    b[i] = norm_param<V>(a.b, group * a.cg + at[i], 0.0f);
+  }
+  const float total = (float)a.cg;
+  for (size_t row = team; row < rows; row += t.teams) {
+    NormVec<V> v[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) v[i] = norm_load<V>(a.x + row * a.cg + at[i]);
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) s += in[i] ? v[i].v[k] : 0.0f;
+    const float mean = norm_row_sums<BLOCK, NT>(s, 0.0f, lanes, wave_sums).x / total;
+    s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        const float d = v[i].v[k] - mean;
+        s = in[i] ? fmaf(d, d, s) : s;
+      }
+    const float rstd = 1.0f / sqrtf(norm_row_sums<BLOCK, NT>(s, 0.0f, lanes, wave_sums).x / total + a.eps);
+    if (lane == 0) {
+      if (a.mean) a.mean[row] = mean;
+      if (a.rstd) a.rstd[row] = rstd;
+    }
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[i].v[k] = norm_out<ACT>(v[i].v[k], mean, rstd, w[i].v[k], b[i].v[k]);
+      if (in[i]) norm_store<V>(a.out + row * a.cg + at[i], v[i]);
+    }
+  }
+}
+
+template <int V, int ACT, int NT, int K, bool BLOCK>
+__global__ __launch_bounds__(NT) void norm_rows_grad_kernel(NormArgs a, NormRows t) {
+  __shared__ float2 wave_sums[NT / 64];
+  const unsigned lanes = BLOCK ? NT : t.lanes, lane = threadIdx.x % lanes, cgv = (unsigned)(a.cg / V);
+  const size_t team = (size_t)blockIdx.x * (NT / lanes) + threadIdx.x / lanes, rows = a.N * a.G;
+  if (team >= t.teams) return;
+  const size_t group = team % a.G;
+  size_t at[K];
+  bool in[K];
+  NormVec<V> w[K], b[K];
+  float s1[K][V], s2[K][V];
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    const unsigned q = lane + i * lanes;
+    in[i] = q < cgv;
+    at[i] = (size_t)(in[i] ? q : cgv - 1) * V;
+    w[i] = norm_param<V>(a.w, group * a.cg + at[i], 1.0f);
+    b[i] = norm_param<V>(a.b, group * a.cg + at[i], 0.0f);
+#pragma unroll
+    for (int k = 0; k < V; ++k) s1[i][k] = s2[i][k] = 0.0f;
+  }
+  const float total = (float)a.cg;
+  NormVec<V> nv[K], ng[K];
+  float nmean = 0.0f, nrstd = 0.0f;
+  auto request = [&](size_t row) {  // the next row while this one is computed (behind the last: the last again)
+    row = row < rows ? row : rows - 1;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      nv[i] = norm_load<V>(a.x + row * a.cg + at[i]);
+      ng[i] = norm_load<V>(a.g + row * a.cg + at[i]);
+    }
+    nmean = a.mean[row];
+    nrstd = a.rstd[row];
+  };
+  request(team);
+  for (size_t row = team; row < rows; row += t.teams) {
+    NormVec<V> v[K], g[K];
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      v[i] = nv[i];
+      g[i] = ng[i];
+    }
+    const float mean = nmean, rstd = nrstd;
+    request(row + t.teams);
+    float ga = 0.0f, gb = 0.0f;
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        float hat;
+        float gu = norm_upstream<ACT>(v[i].v[k], g[i].v[k], mean, rstd, w[i].v[k], b[i].v[k], hat);
+        gu = in[i] ? gu : 0.0f;
+        s1[i][k] += gu;
+        s2[i][k] = fmaf(gu, hat, s2[i][k]);
+        const float gx = gu * w[i].v[k];
+        ga += gx;
+        gb = fmaf(gx, hat, gb);
+        v[i].v[k] = hat;
+        g[i].v[k] = gx;
+      }
+    if (!a.dx) continue;
+    const float2 sums = norm_row_sums<BLOCK, NT>(ga, gb, lanes, wave_sums);
+    ga = sums.x / total;
+    gb = sums.y / total;
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) v[i].v[k] = rstd * (g[i].v[k] - ga - v[i].v[k] * gb);
+      if (in[i]) {
+        float* const o = a.dx + row * a.cg + at[i];
+        if (a.beta != 0.0f) {
+          const NormVec<V> old = norm_load<V>(o);
+#pragma unroll
+          for (int k = 0; k < V; ++k) v[i].v[k] = a.beta * old.v[k] + v[i].v[k];
+        }
+        norm_store<V>(o, v[i]);
+      }
+    }
+  }
+  if (!a.cols) return;
+  float* const o = a.cols + team / a.G * 2 * a.C + group * a.cg;
+#pragma unroll
+  for (int i = 0; i < K; ++i)
+    if (in[i]) {
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        o[at[i] + k] = s2[i][k];
+        o[a.C + at[i] + k] = s1[i][k];
+      }
+    }
 }
 
 // dweight and dbias: the columns of [rows][2][C] summed, 32 columns to a workgroup, 32 rows at a time.
@@ -335,31 +762,126 @@ __global__ __launch_bounds__(1024) void norm_columns_kernel(size_t rows, size_t 
 }
 
 // ---------------------------------------------------------------- host side
-// Cuts every group into windows of channels (a workgroup holds 256 vectors) and runs of positions, such that the chip
-// gets about 2048 workgroups and a thread still 8 positions.
-static void norm_plan(const slhip_ctx* ctx, NormArgs& a, int V, size_t samples) {
+// Windows of about 64 vectors: whole groups, or pieces of one; rows of a workgroup of 256 threads.
+static void norm_windows(NormArgs& a, int V, unsigned threads) {
   const size_t cgv = a.cg / V;
-  a.windows = (unsigned)((cgv + 255) / 256);
-  a.wv = (unsigned)((cgv + a.windows - 1) / a.windows);
-  a.rows = 256 / a.wv;
+  a.together = 1;
+  a.windows = 1;
+  if (cgv > threads) {
+    a.windows = (unsigned)((cgv + threads - 1) / threads);
+    a.lanes = (unsigned)((cgv + a.windows - 1) / a.windows);
+  } else {
+    if (cgv < 64) a.together = (unsigned)(64 / cgv);
+    if (a.together > a.G) a.together = (unsigned)a.G;
+    a.lanes = (unsigned)(a.together * cgv);
+  }
+  a.rows = threads / a.lanes;
   if (a.rows > a.P) a.rows = (unsigned)a.P;
-  const size_t groups = samples * a.G * a.windows, want = (size_t)ctx->num_cu * 8;
+}
+static size_t norm_across(const NormArgs& a) { return (a.G + a.together - 1) / a.together * a.windows; }
+
+// Two pass: runs of positions such that the chip gets about 2048 workgroups and a thread still 8 positions.
+static void norm_plan(const slhip_ctx* ctx, NormArgs& a, int V) {
+  norm_windows(a, V, 256);
+  const size_t groups = a.N * norm_across(a), want = (size_t)ctx->num_cu * 8;
   size_t chunks = (want + groups - 1) / groups;
   const size_t most = (a.P + (size_t)a.rows * 8 - 1) / ((size_t)a.rows * 8);
   if (chunks > most) chunks = most;
-  if (chunks > 256) chunks = 256;
+  if (chunks > 64) chunks = 64;
   if (chunks < 1) chunks = 1;
   a.chunk = (a.P + chunks - 1) / chunks;
   a.chunks = (unsigned)((a.P + a.chunk - 1) / a.chunk);
 }
 
+// On chip: whether a window of whole groups fits a workgroup of `threads` that holds K positions to a thread; as many
+// groups together as fit, up to 64 vectors.
+static bool norm_fits(NormArgs& a, int V, unsigned threads, unsigned K) {
+  const size_t cgv = a.cg / V;
+  if (cgv > threads) return false;
+  a.windows = a.chunks = 1;
+  a.chunk = a.P;
+  a.together = cgv < 64 ? (unsigned)(64 / cgv) : 1;
+  if (a.together > a.G) a.together = (unsigned)a.G;
+  for (; a.together > 0; --a.together) {
+    a.lanes = (unsigned)(a.together * cgv);
+    a.rows = threads / a.lanes;
+    if (a.rows > a.P) a.rows = (unsigned)a.P;
+    if ((size_t)a.rows * K >= a.P) break;
+  }
+  if (a.together == 0) return false;
+  a.blocks = a.N * norm_across(a);
+  return true;
+}
+
+// Rows: the team of a row - K vectors to each of `lanes` threads, in workgroups of NT - and how many teams.
+struct NormTeams {
+  NormRows t;
+  unsigned threads, K;
+  size_t blocks;
+};
+static bool norm_teams(const NormArgs& a, int V, size_t most_vectors, size_t most_blocks, NormTeams* r) {
+  const size_t cgv = a.cg / V;
+  if (cgv > most_vectors) return false;
+  r->K = 2;
+  r->threads = 256;
+  unsigned lanes = 1;
+  if (cgv <= 128) {
+    while (lanes * 2 < cgv) lanes *= 2;
+  } else if (cgv <= 1024) {
+    lanes = 256;
+    r->K = cgv <= 256 ? 1 : cgv <= 512 ? 2 : 4;
+  } else {
+    lanes = r->threads = 1024;
+    r->K = cgv <= 2048 ? 2 : 4;
+  }
+  const size_t in_block = r->threads / lanes, rows = a.N * a.G;
+  r->blocks = (rows + in_block - 1) / in_block;
+  if (r->blocks > most_blocks) r->blocks = most_blocks;
+  const size_t least = (a.G + in_block - 1) / in_block;  // a team for every group
+  if (r->blocks < least) r->blocks = least;
+  if (r->blocks > MAX_GRID) return false;
+  r->t.lanes = lanes;
+  r->t.teams = r->blocks * in_block / a.G * a.G;
+  if (r->t.teams > rows) r->t.teams = rows;  // (a multiple of the groups)
+  return true;
+}
+
+#define NORM_ROWS(KERNEL, NT, K, BLOCK) \
+  hipLaunchKernelGGL((KERNEL<V, ACT, NT, K, BLOCK>), dim3((unsigned)r.blocks), dim3(NT), 0, ctx->stream, a, r.t)
+#define NORM_ROWS_ANY(KERNEL, LAST)                               \
+  do {                                                            \
+    if (r.t.lanes <= 64) NORM_ROWS(KERNEL, 256, 2, false);        \
+    else if (r.threads == 256 && r.K == 1) NORM_ROWS(KERNEL, 256, 1, true); \
+    else if (r.threads == 256 && r.K == 2) NORM_ROWS(KERNEL, 256, 2, true); \
+    else if (r.threads == 256) NORM_ROWS(KERNEL, 256, 4, true);   \
+    else if (r.K == 2) NORM_ROWS(KERNEL, 1024, 2, true);          \
+    else NORM_ROWS(KERNEL, 1024, LAST, true);                     \
+  } while (0)
+
 template <int V, int ACT>
 static int32_t norm_forward(slhip_ctx* ctx, NormArgs a) {
-  norm_plan(ctx, a, V, a.N);
-  const size_t each = a.G * a.windows * a.chunks;  // workgroups of a sample
+  NormTeams r;
+  if (a.P == 1 && norm_teams(a, V, 4096, (size_t)ctx->num_cu * 16, &r)) {
+    NORM_ROWS_ANY(norm_rows_kernel, 4);
+    return post_launch();
+  }
+  // (a few workgroups that hold a large window each would leave most of the chip idle)
+  constexpr unsigned K = V == 4 ? 12 : 16;  // positions of a thread in workgroups of 1024: what 128 registers hold
+  for (const auto& size : {std::pair<unsigned, unsigned>{256, 4}, {256, 16}, {1024, K}}) {
+    if (!norm_fits(a, V, size.first, size.second) || a.blocks > MAX_GRID - 8) continue;
+    if (size.first == 1024 && a.blocks * 4 < (size_t)ctx->num_cu) continue;
+    const dim3 grid((unsigned)((a.blocks + 7) / 8 * 8));
+    if (size.first == 1024) hipLaunchKernelGGL((norm_chip_kernel<V, ACT, 1024, K>), grid, dim3(1024), 0, ctx->stream, a);
+    else if (size.second == 4) hipLaunchKernelGGL((norm_chip_kernel<V, ACT, 256, 4>), grid, dim3(256), 0, ctx->stream, a);
+    else hipLaunchKernelGGL((norm_chip_kernel<V, ACT, 256, 16>), grid, dim3(256), 0, ctx->stream, a);
+    return post_launch();
+  }
+  norm_plan(ctx, a, V);
+  const size_t blocks = norm_across(a) * a.chunks;  // workgroups of a sample
+  const size_t bytes = a.G * a.windows * a.chunks * 2 * sizeof(float);
   // as many samples at a time as the workspace and a launch hold
-  size_t samples = ctx->workspace_bytes / (each * 2 * sizeof(float));
-  if (samples > (MAX_GRID - 8) / each) samples = (MAX_GRID - 8) / each;
+  size_t samples = ctx->workspace_bytes / bytes;
+  if (samples > (MAX_GRID - 8) / blocks) samples = (MAX_GRID - 8) / blocks;
   if (samples == 0) {
     set_error("slhip_group_norm: workspace too small for %zu groups", a.G);
     return SLHIP_EWORKSPACE;
@@ -367,7 +889,7 @@ static int32_t norm_forward(slhip_ctx* ctx, NormArgs a) {
   a.part = (float*)ctx->workspace;
   for (a.n0 = 0; a.n0 < a.N; a.n0 += samples) {
     const size_t k = a.N - a.n0 < samples ? a.N - a.n0 : samples;
-    a.blocks = k * each;
+    a.blocks = k * blocks;
     const dim3 grid((unsigned)((a.blocks + 7) / 8 * 8));
     hipLaunchKernelGGL((norm_stats_kernel<V>), grid, dim3(256), 0, ctx->stream, a);
     int32_t rc = post_launch();
@@ -379,43 +901,67 @@ static int32_t norm_forward(slhip_ctx* ctx, NormArgs a) {
   return SLHIP_OK;
 }
 
+static int32_t norm_columns(slhip_ctx* ctx, size_t rows, size_t C, const float* cols, float* dw, float* db, float beta) {
+  if (!grid_fits(C, 32)) {
+    set_error("slhip_group_norm_grad: too many channels for one launch");
+    return SLHIP_EINVAL;
+  }
+  hipLaunchKernelGGL(norm_columns_kernel, dim3(ceil_div(C, 32)), dim3(1024), 0, ctx->stream, rows, C, cols, dw, db, beta);
+  return post_launch();
+}
+
 template <int V, int ACT>
 static int32_t norm_backward(slhip_ctx* ctx, NormArgs a, float* dw, float* db) {
-  norm_plan(ctx, a, V, a.N);
-  const size_t each = a.G * a.windows * a.chunks;
-  const size_t bytes = (each * 2 + (size_t)a.chunks * 2 * a.C) * sizeof(float);
+  NormTeams r;
+  // two workgroups to a CU: a team then takes many rows, and leaves one row of column sums for all of them
+  if (a.P == 1 && norm_teams(a, V, 2048, (size_t)ctx->num_cu * 2, &r) && r.t.teams / a.G <= ctx->workspace_bytes / (2 * a.C * sizeof(float))) {
+    a.cols = dw || db ? (float*)ctx->workspace : nullptr;
+    NORM_ROWS_ANY(norm_rows_grad_kernel, 2);
+    const int32_t rc = post_launch();
+    return rc || !a.cols ? rc : norm_columns(ctx, r.t.teams / a.G, a.C, a.cols, dw, db, a.beta);
+  }
+  constexpr unsigned K = V == 4 ? 6 : 8;
+  if (a.N <= ctx->workspace_bytes / (2 * a.C * sizeof(float)))
+    for (const auto& size : {std::pair<unsigned, unsigned>{256, 4}, {256, 8}, {1024, K}}) {
+      if (!norm_fits(a, V, size.first, size.second) || a.blocks > MAX_GRID - 8) continue;
+      if (size.first == 1024 && a.blocks * 4 < (size_t)ctx->num_cu) continue;
+      a.cols = dw || db ? (float*)ctx->workspace : nullptr;
+      const dim3 grid((unsigned)((a.blocks + 7) / 8 * 8));
+      if (size.first == 1024) hipLaunchKernelGGL((norm_chip_grad_kernel<V, ACT, 1024, K>), grid, dim3(1024), 0, ctx->stream, a);
+      else if (size.second == 4) hipLaunchKernelGGL((norm_chip_grad_kernel<V, ACT, 256, 4>), grid, dim3(256), 0, ctx->stream, a);
+      else hipLaunchKernelGGL((norm_chip_grad_kernel<V, ACT, 256, 8>), grid, dim3(256), 0, ctx->stream, a);
+      const int32_t rc = post_launch();
+      return rc || !a.cols ? rc : norm_columns(ctx, a.N, a.C, a.cols, dw, db, a.beta);
+    }
+  norm_plan(ctx, a, V);
+  const size_t blocks = norm_across(a) * a.chunks, parts = a.G * a.windows * a.chunks * 2;
+  const size_t bytes = (parts + (size_t)a.chunks * 2 * a.C) * sizeof(float);
   size_t samples = ctx->workspace_bytes / bytes;
-  if (samples > (MAX_GRID - 8) / each) samples = (MAX_GRID - 8) / each;
+  if (samples > (MAX_GRID - 8) / blocks) samples = (MAX_GRID - 8) / blocks;
   if (samples == 0) {
     set_error("slhip_group_norm_grad: workspace too small for %zu channels", a.C);
     return SLHIP_EWORKSPACE;
   }
   if (samples > a.N) samples = a.N;
   a.part = (float*)ctx->workspace;
-  a.cols = dw || db ? a.part + samples * each * 2 : nullptr;
+  a.cols = dw || db ? a.part + samples * parts : nullptr;
   float beta = a.beta;
   for (a.n0 = 0; a.n0 < a.N; a.n0 += samples) {
     const size_t k = a.N - a.n0 < samples ? a.N - a.n0 : samples;
-    a.blocks = k * each;
+    a.blocks = k * blocks;
     const dim3 grid((unsigned)((a.blocks + 7) / 8 * 8));
     hipLaunchKernelGGL((norm_grad_sums_kernel<V, ACT>), grid, dim3(256), 0, ctx->stream, a);
     int32_t rc = post_launch();
     if (rc) return rc;
-    if (a.cols) {
-      if (!grid_fits(a.C, 32)) {
-        set_error("slhip_group_norm_grad: too many channels for one launch");
-        return SLHIP_EINVAL;
-      }
-      hipLaunchKernelGGL(norm_columns_kernel, dim3(ceil_div(a.C, 32)), dim3(1024), 0, ctx->stream, k * a.chunks, a.C, (const float*)a.cols,
-                         dw, db, beta);
-      rc = post_launch();
-      if (rc) return rc;
-      beta = 1.0f;  // further samples add to what these left
-    }
     if (a.dx) {
       hipLaunchKernelGGL((norm_grad_apply_kernel<V, ACT>), grid, dim3(256), 0, ctx->stream, a);
       rc = post_launch();
       if (rc) return rc;
+    }
+    if (a.cols) {
+      rc = norm_columns(ctx, k * a.chunks, a.C, a.cols, dw, db, beta);
+      if (rc) return rc;
+      beta = 1.0f;  // further samples add to what these left
     }
   }
   return SLHIP_OK;
