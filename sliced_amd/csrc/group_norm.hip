@@ -15,7 +15,7 @@
 //            of their own, and the second kernel starts where the first one ended, with what the last-level cache still
 //            holds.
 //
-// In the latter two a window is a run of whole groups, about 64 vectors of channels wide (1 KiB of a row of x): narrower
+// In the latter two a window is a run of whole groups, about 32 vectors of channels wide (512 bytes of a row of x): narrower
 // pieces of rows than that cost HBM bandwidth.  Groups wider than a workgroup are cut.  A thread keeps to one vector of V
 // channels and steps through the positions, so that weights, biases and per-channel sums stay in registers.  V is the
 // widest of 4, 2, 1 that divides a group's channels.
@@ -33,6 +33,7 @@ struct NormArgs {
   unsigned lanes;         // vectors of channels that a workgroup covers
   unsigned together;      // groups of a window, or 1 where a group is cut into
   unsigned windows;       //   this many windows
+  unsigned across;        // windows of a sample
   unsigned rows;          // positions that a workgroup takes at a time
   unsigned chunks;        // runs of positions of a sample, a workgroup each
   size_t chunk;           // positions of a run
@@ -90,6 +91,23 @@ __device__ __forceinline__ NormVec<V> norm_param(const float* p, size_t c, float
   return r;
 }
 
+// The normal distribution's function and density at u, for x * Phi(x) and its slope: erfc by Abramowitz and Stegun's
+// formula 7.1.26 - a polynomial in 1/(1 + p x) times exp(-x^2), off by at most 1.5e-7 - whose exponential is the density's
+// as well.  (The library's erff takes a branch each for small and large arguments, which both run in a wave; with it the
+// arithmetic, not HBM, bounded these kernels: 10 x 961 x 390 forward 17 us.)
+__device__ __forceinline__ float norm_normal(float u, float& density) {
+  const float x = fabsf(u) * 0.70710678118654752f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.0f));
+  const float e = __builtin_amdgcn_exp2f(u * u * -0.72134752044448170f);  // exp(-u^2 / 2)
+  float y = fmaf(1.061405429f, t, -1.453152027f);
+  y = fmaf(y, t, 1.421413741f);
+  y = fmaf(y, t, -0.284496736f);
+  y = fmaf(y, t, 0.254829592f);
+  y = 0.5f * (y * t) * e;  // erfc(x) / 2
+  density = e * 0.39894228040143268f;
+  return u >= 0.0f ? 1.0f - y : y;
+}
+
 template <int ACT>
 __device__ __forceinline__ float norm_act(float u) {
   if (ACT == SLHIP_ACT_RELU) return (u >= 0.0f ? 1.0f : 0.0f) * u;
@@ -98,7 +116,10 @@ __device__ __forceinline__ float norm_act(float u) {
     sigmoid_pair(u, q, rest);
     return u * q;
   }
-  if (ACT == SLHIP_ACT_GELU) return 0.5f * u * (1.0f + erff(u * 0.70710678118654752f));
+  if (ACT == SLHIP_ACT_GELU) {
+    float density;
+    return u * norm_normal(u, density);
+  }
   return u;
 }
 template <int ACT>
@@ -109,8 +130,11 @@ __device__ __forceinline__ float norm_act_grad(float u) {
     sigmoid_pair(u, q, rest);
     return q * (1.0f + u * rest);
   }
-  if (ACT == SLHIP_ACT_GELU)
-    return 0.5f * (1.0f + erff(u * 0.70710678118654752f)) + u * expf(-0.5f * u * u) * 0.39894228040143268f;
+  if (ACT == SLHIP_ACT_GELU) {
+    float density;
+    const float phi = norm_normal(u, density);
+    return fmaf(u, density, phi);
+  }
   return 1.0f;
 }
 // One element of either direction.
@@ -139,41 +163,36 @@ struct NormPlace {
 template <int V, int NT>
 __device__ __forceinline__ NormPlace norm_place(const NormArgs& a, bool backwards) {
   NormPlace p;
-  const size_t per = (a.blocks + 7) / 8;
-  size_t id = (size_t)(blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  p.some = (blockIdx.x >> 3) < per && id < a.blocks;
+  const unsigned blocks = (unsigned)a.blocks, per = (blocks + 7) / 8;
+  unsigned id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  p.some = (blockIdx.x >> 3) < per && id < blocks;
   if (!p.some) id = 0;
-  if (backwards) id = a.blocks - 1 - id;
+  if (backwards) id = blocks - 1 - id;
   const unsigned cgv = (unsigned)(a.cg / V);
-  const size_t across = (a.G + a.together - 1) / a.together;
   p.lane = threadIdx.x % a.lanes;
   p.row = threadIdx.x / a.lanes;
-  const size_t window = id % (across * a.windows);
-  id /= across * a.windows;
-  const unsigned chunk = (unsigned)(id % a.chunks);
+  const unsigned window = id % a.across;
+  id /= a.across;
+  const unsigned chunk = id % a.chunks;
   p.n = a.n0 + id / a.chunks;
   p.active = p.some && p.row < a.rows;
-  size_t v;
+  unsigned v;
   if (a.windows > 1) {
-    const unsigned piece = (unsigned)(window % a.windows);
-    p.g = window / a.windows;
+    const unsigned piece = window % a.windows, group = window / a.windows;
+    p.g = group;
     p.local = 0;
     p.part = chunk * a.windows + piece;
-    v = (size_t)piece * a.lanes + p.lane;
+    v = piece * a.lanes + p.lane;
     p.active = p.active && v < cgv;
-    v = p.g * cgv + (v < cgv ? v : 0);
+    p.c = group * a.cg + (size_t)(v < cgv ? v : 0) * V;
   } else {
     p.local = p.lane / cgv;
-    p.g = window * a.together + p.local;
+    v = window * a.together + p.local;  // the group
     p.part = chunk;
-    p.active = p.active && p.g < a.G;
-    v = window * a.lanes + p.lane;
-    if (p.g >= a.G) {
-      p.g = a.G - 1;
-      v = 0;
-    }
+    p.active = p.active && v < a.G;
+    p.g = v < a.G ? v : a.G - 1;
+    p.c = v < a.G ? ((size_t)window * a.lanes + p.lane) * V : 0;
   }
-  p.c = v * V;
   const size_t begin = (size_t)chunk * a.chunk;
   p.end = begin + a.chunk < a.P ? begin + a.chunk : a.P;
   p.first = begin + p.row;
@@ -190,21 +209,37 @@ __device__ __forceinline__ float norm_count(const NormArgs& a, unsigned part) {
   return (float)((end - begin) * (v1 - v0) * V);
 }
 
-// Sums of two values over the threads of each group of the window: a wave takes the threads of one group at a time, in a
-// fixed order.  Threads without work bring zeros.
+// Sums of two values over the threads of each group of the window, in a fixed order: a wave takes the threads of one group
+// at a time, or, where there is one group only, its own, and then the waves are added up.  Threads without work bring
+// zeros.
 template <int NT>
 struct NormSums {
   float2 value[NT];
   float2 total[64];
+  float reference[64];
 };
 template <int V, int NT>
 __device__ __forceinline__ float2 norm_group_sums(const NormArgs& a, const NormPlace& p, float x, float y, NormSums<NT>& s) {
-  const unsigned cgv = a.windows > 1 ? a.lanes : (unsigned)(a.cg / V), lane = threadIdx.x & 63;
-  __syncthreads();  // the totals of an earlier call have been read
-  s.value[threadIdx.x] = p.active ? make_float2(x, y) : make_float2(0.0f, 0.0f);
+  const unsigned lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  float2 t = p.active ? make_float2(x, y) : make_float2(0.0f, 0.0f);
+  if (a.together == 1) {
+    t.x = wave_reduce<SumOp>(t.x);
+    t.y = wave_reduce<SumOp>(t.y);
+    if (lane == 0) s.total[wave] = t;
+    __syncthreads();
+    t = s.total[0];
+#pragma unroll
+    for (int i = 1; i < NT / 64; ++i) {
+      t.x += s.total[i].x;
+      t.y += s.total[i].y;
+    }
+    return t;
+  }
+  const unsigned cgv = (unsigned)(a.cg / V);
+  s.value[threadIdx.x] = t;
   __syncthreads();
-  for (unsigned k = threadIdx.x >> 6; k < a.together; k += NT / 64) {
-    float2 t = make_float2(0.0f, 0.0f);
+  for (unsigned k = wave; k < a.together; k += NT / 64) {
+    t = make_float2(0.0f, 0.0f);
     for (unsigned i = lane; i < a.rows * cgv; i += 64) {
       const unsigned r = i / cgv;
       const float2 v = s.value[r * a.lanes + k * cgv + (i - r * cgv)];
@@ -231,6 +266,22 @@ __device__ __forceinline__ NormTeam norm_team(const NormArgs& a, const NormPlace
   const unsigned mine = a.windows > 1 ? (cgv - piece * a.lanes < a.lanes ? cgv - piece * a.lanes : a.lanes) : cgv;
   const unsigned lane = a.windows > 1 ? p.lane : p.lane - p.local * cgv;
   return NormTeam{p.row * mine + lane, a.rows * mine};
+}
+
+// Joins what the threads of a group know of it: `count` values of mean `here` whose squared differences from that add up to
+// `spread`.  Means are taken relative to the one of the group's first thread: it is the mean of many values itself, so
+// that no single value, however far from the others, stands between the sums and their difference.
+template <int V, int NT>
+__device__ __forceinline__ void norm_join(const NormArgs& a, const NormPlace& p, unsigned rank, float count, float here, float spread, float total,
+                                          NormSums<NT>& s, float& mean, float& m2) {
+  if (p.active && rank == 0) s.reference[p.local] = here;
+  __syncthreads();
+  const float reference = s.reference[p.local], away = here - reference;
+  const float2 t = norm_group_sums<V, NT>(a, p, count * away, spread + count * (away * away), s);
+  const float shift = t.x / total;
+  mean = reference + shift;
+  m2 = fmaxf(t.y - t.x * shift, 0.0f);
+  if (t.y != t.y) m2 = t.y;  // (fmaxf would lose a NaN)
 }
 
 // A thread's sums over its positions, 4 of them requested at a time.
@@ -268,12 +319,10 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormArgs a) {
     count += (float)(U * V);
   });
   const float m = count > 0.0f ? s1 / count : 0.0f;
-  const float here = shift + m;                   // the thread's mean
-  const float spread = fmaxf(s2 - s1 * m, 0.0f);  // and its sum of squared differences
-  const float mean = norm_group_sums<V, 256>(a, p, count * here, 0.0f, sums).x / norm_count<V>(a, p.part);
-  const float away = here - mean;
-  const float m2 = norm_group_sums<V, 256>(a, p, spread + count * (away * away), 0.0f, sums).x;
-  if (p.active && norm_team<V>(a, p).rank == 0) {
+  const unsigned rank = norm_team<V>(a, p).rank;
+  float mean, m2;
+  norm_join<V, 256>(a, p, rank, count, shift + m, s2 - s1 * m, norm_count<V>(a, p.part), sums, mean, m2);
+  if (p.active && rank == 0) {
     float* o = a.part + 2 * (((p.n - a.n0) * a.G + p.g) * (a.chunks * a.windows) + p.part);
     o[0] = mean;
     o[1] = m2;
@@ -290,15 +339,18 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormArgs a) {
   const float* in = a.part + 2 * ((p.n - a.n0) * a.G + p.g) * parts;
   const float total = (float)(a.P * a.cg);
   const NormTeam t = norm_team<V>(a, p);
-  float s = 0.0f;
-  for (unsigned i = t.rank; i < parts; i += t.size) s += norm_count<V>(a, i) * in[2 * i];
-  const float mean = norm_group_sums<V, 256>(a, p, s, 0.0f, sums).x / total;
-  s = 0.0f;
+  const float reference = in[0];
+  float s1 = 0.0f, s2 = 0.0f;
   for (unsigned i = t.rank; i < parts; i += t.size) {
-    const float away = in[2 * i] - mean;
-    s += in[2 * i + 1] + norm_count<V>(a, i) * (away * away);
+    const float count = norm_count<V>(a, i), away = in[2 * i] - reference;
+    s1 = fmaf(count, away, s1);
+    s2 += fmaf(count, away * away, in[2 * i + 1]);
   }
-  const float rstd = 1.0f / sqrtf(norm_group_sums<V, 256>(a, p, s, 0.0f, sums).x / total + a.eps);
+  const float2 both = norm_group_sums<V, 256>(a, p, s1, s2, sums);
+  const float mean = reference + both.x / total;
+  float var = (both.y - both.x * (both.x / total)) / total;
+  if (var < 0.0f) var = 0.0f;
+  const float rstd = 1.0f / sqrtf(var + a.eps);
   if (!p.active) return;
   if (p.part == 0 && t.rank == 0) {
     if (a.mean) a.mean[p.n * a.G + p.g] = mean;
@@ -445,8 +497,7 @@ __global__ __launch_bounds__(256) void norm_grad_apply_kernel(NormArgs a) {
 }
 
 // ---------------------------------------------------------------- on chip
-// All P <= rows * K positions of a window in the registers of one workgroup: the variance from differences to the mean
-// itself, x read once.
+// All P <= rows * K positions of a window in the registers of one workgroup: x is read once.
 template <int V, int ACT, int NT, int K>
 __global__ __launch_bounds__(NT) void norm_chip_kernel(NormArgs a) {
   __shared__ NormSums<NT> sums;
@@ -459,30 +510,36 @@ __global__ __launch_bounds__(NT) void norm_chip_kernel(NormArgs a) {
     const size_t r = p.row + (size_t)i * a.rows;
     v[i] = norm_load<V>(a.x + base + (r < a.P ? r : a.P - 1) * a.C);
   }
+  // the thread's own mean, and its squared differences from that
   const float total = (float)(a.P * a.cg);
-  float s = 0.0f;
+  float count = 0.0f, s = 0.0f;
 #pragma unroll
   for (int i = 0; i < K; ++i) {
+    const bool in = p.row + (size_t)i * a.rows < a.P;
     float t = 0.0f;
 #pragma unroll
     for (int k = 0; k < V; ++k) t += v[i].v[k];
-    s += p.row + (size_t)i * a.rows < a.P ? t : 0.0f;
+    s += in ? t : 0.0f;
+    count += in ? (float)V : 0.0f;
   }
-  const float mean = norm_group_sums<V, NT>(a, p, s, 0.0f, sums).x / total;
+  const float here = count > 0.0f ? s / count : 0.0f;
   s = 0.0f;
 #pragma unroll
   for (int i = 0; i < K; ++i) {
     float t = 0.0f;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
-      const float d = v[i].v[k] - mean;
+      const float d = v[i].v[k] - here;
       t = fmaf(d, d, t);
     }
     s += p.row + (size_t)i * a.rows < a.P ? t : 0.0f;
   }
-  const float rstd = 1.0f / sqrtf(norm_group_sums<V, NT>(a, p, s, 0.0f, sums).x / total + a.eps);
+  const unsigned rank = norm_team<V>(a, p).rank;
+  float mean, m2;
+  norm_join<V, NT>(a, p, rank, count, here, s, total, sums, mean, m2);
+  const float rstd = 1.0f / sqrtf(m2 / total + a.eps);
   if (!p.active) return;
-  if (norm_team<V>(a, p).rank == 0) {
+  if (rank == 0) {
     if (a.mean) a.mean[p.n * a.G + p.g] = mean;
     if (a.rstd) a.rstd[p.n * a.G + p.g] = rstd;
   }
@@ -567,6 +624,7 @@ __global__ __launch_bounds__(NT) void norm_chip_grad_kernel(NormArgs a) {
 // gradients, stays the same.
 struct NormRows {
   unsigned lanes;
+  unsigned fold;  // teams of each group in a workgroup whose column sums are added up there; 1: every team writes its own
   size_t teams;
 };
 
@@ -649,7 +707,7 @@ __global__ __launch_bounds__(NT) void norm_rows_grad_kernel(NormArgs a, NormRows
   __shared__ float2 wave_sums[NT / 64];
   const unsigned lanes = BLOCK ? NT : t.lanes, lane = threadIdx.x % lanes, cgv = (unsigned)(a.cg / V);
   const size_t team = (size_t)blockIdx.x * (NT / lanes) + threadIdx.x / lanes, rows = a.N * a.G;
-  if (team >= t.teams) return;
+  if (t.fold == 1 && team >= t.teams) return;
   const size_t group = team % a.G;
   size_t at[K];
   bool in[K];
@@ -724,7 +782,38 @@ __global__ __launch_bounds__(NT) void norm_rows_grad_kernel(NormArgs a, NormRows
     }
   }
   if (!a.cols) return;
-  float* const o = a.cols + team / a.G * 2 * a.C + group * a.cg;
+  size_t line = team / a.G;
+  if (!BLOCK && t.fold > 1) {
+    // the workgroup's `fold` teams of every group leave one line: a tree over them
+    __shared__ float sums[BLOCK ? 1 : NT][2 * K * V + 1];
+    const unsigned place = threadIdx.x / lanes / (unsigned)a.G, apart = (unsigned)a.G * lanes;
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        sums[threadIdx.x][2 * (i * V + k)] = s1[i][k];
+        sums[threadIdx.x][2 * (i * V + k) + 1] = s2[i][k];
+      }
+    unsigned half = 1;
+    while (half < t.fold) half *= 2;
+    for (half /= 2; half > 0; half /= 2) {
+      __syncthreads();
+      if (place < half && place + half < t.fold) {
+#pragma unroll
+        for (int k = 0; k < 2 * K * V; ++k) sums[threadIdx.x][k] += sums[threadIdx.x + half * apart][k];
+      }
+    }
+    if (place > 0) return;
+#pragma unroll
+    for (int i = 0; i < K; ++i)
+#pragma unroll
+      for (int k = 0; k < V; ++k) {
+        s1[i][k] = sums[threadIdx.x][2 * (i * V + k)];
+        s2[i][k] = sums[threadIdx.x][2 * (i * V + k) + 1];
+      }
+    line = blockIdx.x;
+  }
+  float* const o = a.cols + line * 2 * a.C + group * a.cg;
 #pragma unroll
   for (int i = 0; i < K; ++i)
     if (in[i]) {
@@ -762,7 +851,8 @@ __global__ __launch_bounds__(1024) void norm_columns_kernel(size_t rows, size_t 
 }
 
 // ---------------------------------------------------------------- host side
-// Windows of about 64 vectors: whole groups, or pieces of one; rows of a workgroup of 256 threads.
+// Windows of about NORM_WINDOW vectors: whole groups, or pieces of one.
+constexpr size_t NORM_WINDOW = 32;
 static void norm_windows(NormArgs& a, int V, unsigned threads) {
   const size_t cgv = a.cg / V;
   a.together = 1;
@@ -771,19 +861,19 @@ static void norm_windows(NormArgs& a, int V, unsigned threads) {
     a.windows = (unsigned)((cgv + threads - 1) / threads);
     a.lanes = (unsigned)((cgv + a.windows - 1) / a.windows);
   } else {
-    if (cgv < 64) a.together = (unsigned)(64 / cgv);
+    if (cgv < NORM_WINDOW) a.together = (unsigned)(NORM_WINDOW / cgv);
     if (a.together > a.G) a.together = (unsigned)a.G;
     a.lanes = (unsigned)(a.together * cgv);
   }
+  a.across = (unsigned)((a.G + a.together - 1) / a.together * a.windows);
   a.rows = threads / a.lanes;
   if (a.rows > a.P) a.rows = (unsigned)a.P;
 }
-static size_t norm_across(const NormArgs& a) { return (a.G + a.together - 1) / a.together * a.windows; }
 
-// Two pass: runs of positions such that the chip gets about 2048 workgroups and a thread still 8 positions.
+// Two pass: runs of positions such that the chip gets about 4096 workgroups and a thread still 8 positions.
 static void norm_plan(const slhip_ctx* ctx, NormArgs& a, int V) {
   norm_windows(a, V, 256);
-  const size_t groups = a.N * norm_across(a), want = (size_t)ctx->num_cu * 8;
+  const size_t groups = a.N * a.across, want = (size_t)ctx->num_cu * 16;
   size_t chunks = (want + groups - 1) / groups;
   const size_t most = (a.P + (size_t)a.rows * 8 - 1) / ((size_t)a.rows * 8);
   if (chunks > most) chunks = most;
@@ -793,23 +883,24 @@ static void norm_plan(const slhip_ctx* ctx, NormArgs& a, int V) {
   a.chunks = (unsigned)((a.P + a.chunk - 1) / a.chunk);
 }
 
-// On chip: whether a window of whole groups fits a workgroup of `threads` that holds K positions to a thread; as many
-// groups together as fit, up to 64 vectors.
-static bool norm_fits(NormArgs& a, int V, unsigned threads, unsigned K) {
+// On chip: whether a window of whole groups fits a workgroup of `threads` that holds K positions to a thread.  As many groups
+// together as fit, up to NORM_WINDOW vectors, but no more than leave a workgroup to every CU.
+static bool norm_fits(const slhip_ctx* ctx, NormArgs& a, int V, unsigned threads, unsigned K) {
   const size_t cgv = a.cg / V;
   if (cgv > threads) return false;
   a.windows = a.chunks = 1;
   a.chunk = a.P;
-  a.together = cgv < 64 ? (unsigned)(64 / cgv) : 1;
+  a.together = cgv < NORM_WINDOW ? (unsigned)(NORM_WINDOW / cgv) : 1;
   if (a.together > a.G) a.together = (unsigned)a.G;
   for (; a.together > 0; --a.together) {
     a.lanes = (unsigned)(a.together * cgv);
     a.rows = threads / a.lanes;
     if (a.rows > a.P) a.rows = (unsigned)a.P;
-    if ((size_t)a.rows * K >= a.P) break;
+    a.across = (unsigned)((a.G + a.together - 1) / a.together);
+    if ((size_t)a.rows * K >= a.P && (a.together == 1 || a.N * a.across >= (size_t)ctx->num_cu)) break;
   }
   if (a.together == 0) return false;
-  a.blocks = a.N * norm_across(a);
+  a.blocks = a.N * a.across;
   return true;
 }
 
@@ -817,7 +908,7 @@ static bool norm_fits(NormArgs& a, int V, unsigned threads, unsigned K) {
 struct NormTeams {
   NormRows t;
   unsigned threads, K;
-  size_t blocks;
+  size_t blocks, lines;  // workgroups; lines of column sums that they leave
 };
 static bool norm_teams(const NormArgs& a, int V, size_t most_vectors, size_t most_blocks, NormTeams* r) {
   const size_t cgv = a.cg / V;
@@ -843,6 +934,8 @@ static bool norm_teams(const NormArgs& a, int V, size_t most_vectors, size_t mos
   r->t.lanes = lanes;
   r->t.teams = r->blocks * in_block / a.G * a.G;
   if (r->t.teams > rows) r->t.teams = rows;  // (a multiple of the groups)
+  r->t.fold = lanes <= 64 && in_block % a.G == 0 && in_block / a.G > 1 ? (unsigned)(in_block / a.G) : 1;
+  r->lines = r->t.fold > 1 ? r->blocks : r->t.teams / a.G;
   return true;
 }
 
@@ -868,7 +961,7 @@ static int32_t norm_forward(slhip_ctx* ctx, NormArgs a) {
   // (a few workgroups that hold a large window each would leave most of the chip idle)
   constexpr unsigned K = V == 4 ? 12 : 16;  // positions of a thread in workgroups of 1024: what 128 registers hold
   for (const auto& size : {std::pair<unsigned, unsigned>{256, 4}, {256, 16}, {1024, K}}) {
-    if (!norm_fits(a, V, size.first, size.second) || a.blocks > MAX_GRID - 8) continue;
+    if (!norm_fits(ctx, a, V, size.first, size.second) || a.blocks > MAX_GRID - 8) continue;
     if (size.first == 1024 && a.blocks * 4 < (size_t)ctx->num_cu) continue;
     const dim3 grid((unsigned)((a.blocks + 7) / 8 * 8));
     if (size.first == 1024) hipLaunchKernelGGL((norm_chip_kernel<V, ACT, 1024, K>), grid, dim3(1024), 0, ctx->stream, a);
@@ -877,7 +970,7 @@ static int32_t norm_forward(slhip_ctx* ctx, NormArgs a) {
     return post_launch();
   }
   norm_plan(ctx, a, V);
-  const size_t blocks = norm_across(a) * a.chunks;  // workgroups of a sample
+  const size_t blocks = (size_t)a.across * a.chunks;  // workgroups of a sample
   const size_t bytes = a.G * a.windows * a.chunks * 2 * sizeof(float);
   // as many samples at a time as the workspace and a launch hold
   size_t samples = ctx->workspace_bytes / bytes;
@@ -914,16 +1007,16 @@ template <int V, int ACT>
 static int32_t norm_backward(slhip_ctx* ctx, NormArgs a, float* dw, float* db) {
   NormTeams r;
   // two workgroups to a CU: a team then takes many rows, and leaves one row of column sums for all of them
-  if (a.P == 1 && norm_teams(a, V, 2048, (size_t)ctx->num_cu * 2, &r) && r.t.teams / a.G <= ctx->workspace_bytes / (2 * a.C * sizeof(float))) {
+  if (a.P == 1 && norm_teams(a, V, 2048, (size_t)ctx->num_cu * 2, &r) && r.lines <= ctx->workspace_bytes / (2 * a.C * sizeof(float))) {
     a.cols = dw || db ? (float*)ctx->workspace : nullptr;
     NORM_ROWS_ANY(norm_rows_grad_kernel, 2);
     const int32_t rc = post_launch();
-    return rc || !a.cols ? rc : norm_columns(ctx, r.t.teams / a.G, a.C, a.cols, dw, db, a.beta);
+    return rc || !a.cols ? rc : norm_columns(ctx, r.lines, a.C, a.cols, dw, db, a.beta);
   }
   constexpr unsigned K = V == 4 ? 6 : 8;
   if (a.N <= ctx->workspace_bytes / (2 * a.C * sizeof(float)))
     for (const auto& size : {std::pair<unsigned, unsigned>{256, 4}, {256, 8}, {1024, K}}) {
-      if (!norm_fits(a, V, size.first, size.second) || a.blocks > MAX_GRID - 8) continue;
+      if (!norm_fits(ctx, a, V, size.first, size.second) || a.blocks > MAX_GRID - 8) continue;
       if (size.first == 1024 && a.blocks * 4 < (size_t)ctx->num_cu) continue;
       a.cols = dw || db ? (float*)ctx->workspace : nullptr;
       const dim3 grid((unsigned)((a.blocks + 7) / 8 * 8));
@@ -934,7 +1027,7 @@ static int32_t norm_backward(slhip_ctx* ctx, NormArgs a, float* dw, float* db) {
       return rc || !a.cols ? rc : norm_columns(ctx, a.N, a.C, a.cols, dw, db, a.beta);
     }
   norm_plan(ctx, a, V);
-  const size_t blocks = norm_across(a) * a.chunks, parts = a.G * a.windows * a.chunks * 2;
+  const size_t blocks = (size_t)a.across * a.chunks, parts = a.G * a.windows * a.chunks * 2;
   const size_t bytes = (parts + (size_t)a.chunks * 2 * a.C) * sizeof(float);
   size_t samples = ctx->workspace_bytes / bytes;
   if (samples > (MAX_GRID - 8) / blocks) samples = (MAX_GRID - 8) / blocks;
