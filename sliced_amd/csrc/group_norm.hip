@@ -624,6 +624,7 @@ __global__ __launch_bounds__(NT) void norm_chip_grad_kernel(NormArgs a) {
 // gradients, stays the same.
 struct NormRows {
   unsigned lanes;
+  unsigned used;  // teams of a workgroup: as many as are whole rounds of the groups, if there is one
   unsigned fold;  // teams of each group in a workgroup whose column sums are added up there; 1: every team writes its own
   size_t teams;
 };
@@ -655,8 +656,9 @@ template <int V, int ACT, int NT, int K, bool BLOCK>
 __global__ __launch_bounds__(NT) void norm_rows_kernel(NormArgs a, NormRows t) {
   __shared__ float2 wave_sums[NT / 64];
   const unsigned lanes = BLOCK ? NT : t.lanes, lane = threadIdx.x % lanes, cgv = (unsigned)(a.cg / V);
-  const size_t team = (size_t)blockIdx.x * (NT / lanes) + threadIdx.x / lanes, rows = a.N * a.G;
-  if (team >= t.teams) return;
+  const unsigned local = BLOCK ? 0 : threadIdx.x / lanes;
+  const size_t team = (size_t)blockIdx.x * t.used + local, rows = a.N * a.G;
+  if (local >= t.used || team >= t.teams) return;
   const size_t group = team % a.G;
   size_t at[K];  // of a vector within the row; one past the end stands at the last and is left out
   bool in[K];
@@ -706,9 +708,14 @@ template <int V, int ACT, int NT, int K, bool BLOCK>
 __global__ __launch_bounds__(NT) void norm_rows_grad_kernel(NormArgs a, NormRows t) {
   __shared__ float2 wave_sums[NT / 64];
   const unsigned lanes = BLOCK ? NT : t.lanes, lane = threadIdx.x % lanes, cgv = (unsigned)(a.cg / V);
-  const size_t team = (size_t)blockIdx.x * (NT / lanes) + threadIdx.x / lanes, rows = a.N * a.G;
-  if (t.fold == 1 && team >= t.teams) return;
+  const unsigned local = BLOCK ? 0 : threadIdx.x / lanes;
+  const size_t rows = a.N * a.G;
+  size_t team = (size_t)blockIdx.x * t.used + local;
   const size_t group = team % a.G;
+  if (local >= t.used || team >= t.teams) {
+    if (t.fold == 1) return;
+    team = rows;  // nothing to take, but there for the tree
+  }
   size_t at[K];
   bool in[K];
   NormVec<V> w[K], b[K];
@@ -782,11 +789,11 @@ __global__ __launch_bounds__(NT) void norm_rows_grad_kernel(NormArgs a, NormRows
     }
   }
   if (!a.cols) return;
-  size_t line = team / a.G;
+  size_t line = BLOCK || t.fold == 1 ? team / a.G : 0;
   if (!BLOCK && t.fold > 1) {
     // the workgroup's `fold` teams of every group leave one line: a tree over them
     __shared__ float sums[BLOCK ? 1 : NT][2 * K * V + 1];
-    const unsigned place = threadIdx.x / lanes / (unsigned)a.G, apart = (unsigned)a.G * lanes;
+    const unsigned place = local / (unsigned)a.G, apart = (unsigned)a.G * lanes;
 #pragma unroll
     for (int i = 0; i < K; ++i)
 #pragma unroll
@@ -825,28 +832,39 @@ __global__ __launch_bounds__(NT) void norm_rows_grad_kernel(NormArgs a, NormRows
     }
 }
 
-// dweight and dbias: the columns of [rows][2][C] summed, 32 columns to a workgroup, 32 rows at a time.
+// dweight and dbias: the sums of the 2 * C columns of [rows][2][C].  A workgroup takes 32 columns, eight lanes of four to a
+// row, 128 rows at a time, and adds up what its rows' threads have in LDS, a wave to a column.
 __global__ __launch_bounds__(1024) void norm_columns_kernel(size_t rows, size_t C, const float* __restrict__ cols, float* dw, float* db,
                                                             float beta) {
-  __shared__ float sw[32][33], sb[32][33];
-  const unsigned lane = threadIdx.x & 31, slot = threadIdx.x >> 5;
-  const size_t c = (size_t)blockIdx.x * 32 + lane;
-  float x = 0.0f, y = 0.0f;
-  if (c < C) {
+  __shared__ float sums[128][33];
+  const unsigned lane = threadIdx.x & 7, slot = threadIdx.x >> 3;
+  const size_t first = (size_t)blockIdx.x * 32, c = first + 4 * lane, width = 2 * C;
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (c + 3 < width) {
 #pragma unroll 4
-    for (size_t r = slot; r < rows; r += 32) {
-      x += cols[2 * r * C + c];
-      y += cols[(2 * r + 1) * C + c];
+    for (size_t r = slot; r < rows; r += 128) {
+      const float4 v = ld4g(cols + r * width + c);
+      s[0] += v.x; s[1] += v.y; s[2] += v.z; s[3] += v.w;
     }
+  } else {
+    for (size_t r = slot; r < rows; r += 128)
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (c + k < width) s[k] += cols[r * width + c + k];
   }
-  sw[slot][lane] = x;
-  sb[slot][lane] = y;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) sums[slot][4 * lane + k] = s[k];
   __syncthreads();
-  if (slot < 2) {
-    float s = 0.0f;
-    for (int k = 0; k < 32; ++k) s += slot == 0 ? sw[k][lane] : sb[k][lane];
-    float* const o = slot == 0 ? dw : db;
-    if (c < C && o) o[c] = beta != 0.0f ? beta * o[c] + s : s;
+  const unsigned half = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (unsigned k = 0; k < 2; ++k) {
+    const unsigned q = wave + 16 * k;
+    const float t = wave_reduce<SumOp>(sums[half][q] + sums[half + 64][q]);
+    const size_t at = first + q;
+    if (half != 0 || at >= width) continue;
+    float* const o = at < C ? dw : db;
+    const size_t e = at < C ? at : at - C;
+    if (o) o[e] = beta != 0.0f ? beta * o[e] + t : t;
   }
 }
 
@@ -926,15 +944,17 @@ static bool norm_teams(const NormArgs& a, int V, size_t most_vectors, size_t mos
     r->K = cgv <= 2048 ? 2 : 4;
   }
   const size_t in_block = r->threads / lanes, rows = a.N * a.G;
-  r->blocks = (rows + in_block - 1) / in_block;
+  r->t.lanes = lanes;
+  r->t.fold = in_block >= 2 * a.G ? (unsigned)(in_block / a.G) : 1;
+  r->t.used = (unsigned)(in_block >= a.G ? in_block / a.G * a.G : in_block);
+  if (r->threads == 1024) most_blocks = (most_blocks + 1) / 2;  // (one of them to a CU)
+  r->blocks = (rows + r->t.used - 1) / r->t.used;
   if (r->blocks > most_blocks) r->blocks = most_blocks;
-  const size_t least = (a.G + in_block - 1) / in_block;  // a team for every group
+  const size_t least = (a.G + r->t.used - 1) / r->t.used;  // a team for every group
   if (r->blocks < least) r->blocks = least;
   if (r->blocks > MAX_GRID) return false;
-  r->t.lanes = lanes;
-  r->t.teams = r->blocks * in_block / a.G * a.G;
+  r->t.teams = r->blocks * r->t.used / a.G * a.G;
   if (r->t.teams > rows) r->t.teams = rows;  // (a multiple of the groups)
-  r->t.fold = lanes <= 64 && in_block % a.G == 0 && in_block / a.G > 1 ? (unsigned)(in_block / a.G) : 1;
   r->lines = r->t.fold > 1 ? r->blocks : r->t.teams / a.G;
   return true;
 }
@@ -995,11 +1015,11 @@ static int32_t norm_forward(slhip_ctx* ctx, NormArgs a) {
 }
 
 static int32_t norm_columns(slhip_ctx* ctx, size_t rows, size_t C, const float* cols, float* dw, float* db, float beta) {
-  if (!grid_fits(C, 32)) {
+  if (!grid_fits(C, 16)) {
     set_error("slhip_group_norm_grad: too many channels for one launch");
     return SLHIP_EINVAL;
   }
-  hipLaunchKernelGGL(norm_columns_kernel, dim3(ceil_div(C, 32)), dim3(1024), 0, ctx->stream, rows, C, cols, dw, db, beta);
+  hipLaunchKernelGGL(norm_columns_kernel, dim3(ceil_div(2 * C, 32)), dim3(1024), 0, ctx->stream, rows, C, cols, dw, db, beta);
   return post_launch();
 }
 
