@@ -284,12 +284,13 @@ __device__ __forceinline__ void norm_join(const NormArgs& a, const NormPlace& p,
   if (t.y != t.y) m2 = t.y;  // (fmaxf would lose a NaN)
 }
 
-// A thread's sums over its positions, 4 of them requested at a time.
+// A thread's positions, several of them requested at a time: 64 bytes of each array, or 32 of narrow vectors.
 template <int V, class F>
 __device__ __forceinline__ void norm_each(const NormArgs& a, const NormPlace& p, F&& f) {
+  constexpr int U = V == 4 ? 4 : 8;
   const size_t step = (size_t)a.rows * a.C;
   size_t at = (p.n * a.P + p.first) * a.C + p.c, r = p.first;
-  for (; r + 3 * (size_t)a.rows < p.end; r += 4 * (size_t)a.rows, at += 4 * step) f(at, step, std::integral_constant<int, 4>());
+  for (; r + (U - 1) * (size_t)a.rows < p.end; r += U * (size_t)a.rows, at += U * step) f(at, step, std::integral_constant<int, U>());
   for (; r < p.end; r += a.rows, at += step) f(at, step, std::integral_constant<int, 1>());
 }
 
@@ -918,6 +919,10 @@ static bool norm_fits(const slhip_ctx* ctx, NormArgs& a, int V, unsigned threads
     if ((size_t)a.rows * K >= a.P && (a.together == 1 || a.N * a.across >= (size_t)ctx->num_cu)) break;
   }
   if (a.together == 0) return false;
+  // Pieces of rows below 96 bytes cost more than the second reading does, unless all of it stays in the caches (forward at 64 x
+  // 2048 x 320 in 32 groups, 40 bytes: 230 us here, 129 in two passes; 10 x 961 x 390 in 13, 120 bytes: 12 and 16; 32 x 1000 x
+  // 64 in 8, 32 bytes but 8 MiB in all: 8 and 14).
+  if (a.across > 1 && a.lanes * (size_t)V < 24 && a.N * a.P * a.C > (size_t(1) << 22)) return false;
   a.blocks = a.N * a.across;
   return true;
 }
