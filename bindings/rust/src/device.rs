@@ -114,6 +114,50 @@ impl<Mods> HIP<Mods> {
 }
 
 impl<Mods> HIP<Mods> {
+    /// One AdamW step of a whole parameter list, its moments in f32.  `counter` names a 64-bit count on
+    /// the device that the call advances, so that a recorded step counts on when it is replayed.
+    #[allow(clippy::too_many_arguments)]
+    pub fn adamw_step<S: Shape>(
+        &self,
+        params: &mut [&mut Buffer<f32, Self, S>],
+        m: &mut [&mut Buffer<f32, Self, S>],
+        v: &mut [&mut Buffer<f32, Self, S>],
+        counter: *mut u64,
+        lr: f32,
+        beta1: f32,
+        beta2: f32,
+        eps: f32,
+        weight_decay: f32,
+    ) where
+        Self: Device,
+    {
+        assert!(m.len() == params.len() && v.len() == params.len());
+        let ps: Vec<*mut f32> = params.iter_mut().map(|p| p.ptr_mut()).collect();
+        let gs: Vec<*const f32> = params.iter().map(|p| p.grad().ptr()).collect();
+        let ms: Vec<*mut f32> = m.iter_mut().map(|p| p.ptr_mut()).collect();
+        let vs: Vec<*mut f32> = v.iter_mut().map(|p| p.ptr_mut()).collect();
+        let ns: Vec<usize> = params.iter().map(|p| p.len()).collect();
+        check(unsafe {
+            ffi::slhip_adamw_step_multi(
+                self.ctx,
+                ps.len(),
+                ps.as_ptr(),
+                gs.as_ptr(),
+                ms.as_ptr(),
+                vs.as_ptr(),
+                ns.as_ptr(),
+                lr,
+                beta1,
+                beta2,
+                eps,
+                weight_decay,
+                0,
+                counter,
+            )
+        })
+        .unwrap();
+    }
+
     /// One whole training step of the sine-fit loop (examples/sine_net.rs:119-166) as two launches:
     /// forward through three Linear layers with ReLU between them, the MSE loss into `loss[0]`,
     /// backward and SGD on the six parameter buffers in place; their gradient buffers receive the

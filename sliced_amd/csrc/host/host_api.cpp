@@ -243,6 +243,46 @@ SLH_API int slh_softmax(void* dev, size_t samples, size_t features, uint64_t x, 
     *out = d->softmax(samples, features, d->lookup(x)).id;
   });
 }
+// weight, bias and h0 may be 0: none
+SLH_API int slh_group_norm(void* dev, size_t samples, size_t positions, size_t channels, size_t groups, uint64_t x, uint64_t weight,
+                           uint64_t bias, int act, float eps, uint64_t* out) {
+  return guard([&] {
+    HIP* d = (HIP*)dev;
+    *out = d->group_norm(samples, positions, channels, groups, d->lookup(x), weight ? d->lookup(weight) : Buffer(),
+                         bias ? d->lookup(bias) : Buffer(), act, eps).id;
+  });
+}
+SLH_API int slh_gated_scan(void* dev, int mode, size_t batch, size_t steps, size_t channels, uint64_t gate, uint64_t x, uint64_t h0,
+                           uint64_t* out) {
+  return guard([&] {
+    HIP* d = (HIP*)dev;
+    *out = d->gated_scan(mode, batch, steps, channels, d->lookup(gate), d->lookup(x), h0 ? d->lookup(h0) : Buffer()).id;
+  });
+}
+SLH_API int slh_gated_scan_step(void* dev, int mode, size_t batch, size_t channels, uint64_t gate, uint64_t x, uint64_t state) {
+  return guard([&] {
+    HIP* d = (HIP*)dev;
+    d->gated_scan_step(mode, batch, channels, d->lookup(gate), d->lookup(x), d->lookup(state));
+  });
+}
+// An AdamW optimiser over `count` buffers; to be freed before the device is.
+SLH_API int slh_adamw_new(void* dev, size_t count, const uint64_t* params, float lr, float beta1, float beta2, float eps, float weight_decay,
+                          int eight, uint64_t seed, void** opt) {
+  return guard([&] {
+    HIP* d = (HIP*)dev;
+    std::vector<Buffer> ps;
+    for (size_t i = 0; i < count; ++i) ps.push_back(d->lookup(params[i]));
+    HIP::AdamWRates r;
+    r.lr = lr; r.beta1 = beta1; r.beta2 = beta2; r.eps = eps; r.weight_decay = weight_decay;
+    *opt = new AdamW(*d, ps, r, eight != 0, seed);
+  });
+}
+SLH_API int slh_adamw_step(void* opt) {
+  return guard([&] { ((AdamW*)opt)->step(); });
+}
+SLH_API int slh_adamw_free(void* opt) {
+  return guard([&] { delete (AdamW*)opt; });
+}
 // kind: 0 sum_rows, 1 sum_cols, 2 max_rows, 3 max_cols, 4 mean_rows, 5 mean_cols
 SLH_API int slh_reduce(void* dev, int kind, size_t rows, size_t cols, uint64_t x, uint64_t* out) {
   return guard([&] {
@@ -269,7 +309,7 @@ SLH_API int slh_sgd_step(void* dev, uint64_t p, float lr) {
 // kind 0 = sine fit (MSE on the tape), 1 = classifier (softmax + cce).  W1..b3 are updated in
 // place.  `warmup` untimed steps run first (they train too); seconds = wall time of `steps`.
 // mode: bit 0 = fused Linear forward, bit 1 = record one step as a graph and replay it,
-// bit 2 = fused loss kernels.
+// bit 2 = fused loss kernels, bit 4 = AdamW instead of SGD, bit 5 = AdamW with 8-bit moments.
 SLH_API int slh_mlp_train(int ordinal, int kind, size_t batch, size_t d_in, size_t d_h, size_t d_out, const float* x,
                           const float* target, float* W1, float* b1, float* W2, float* b2, float* W3, float* b3,
                           float lr, size_t steps, size_t warmup, int mode, float* losses, double* seconds,

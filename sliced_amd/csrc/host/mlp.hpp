@@ -2,11 +2,13 @@
 // API exactly as the examples are written against Matrix / CPU:
 //   Linear { weights, bias }   forward = gemm + add_row_mut          examples/sine_net.rs:8-48
 //   SGD                         value -= grad * lr                     examples/sine_net.rs:80-117
+//   AdamW                       beside it (no counterpart in the reference)
 //   sine fit (kind 0)           examples/sine_net.rs:119-166
 //   classifier (kind 1)         examples/nn.rs:154-244, cce / cce_grad :124-152
 // Everything stays on the device; per step the host reads back one float (the loss).
 #pragma once
 #include <chrono>
+#include <memory>
 
 #include "sliced.hpp"
 
@@ -50,6 +52,38 @@ struct SGD {
   }
 };
 
+// AdamW over a parameter list, with its moments in f32 or in 8 bits and its count of steps on the device.
+class AdamW {
+ public:
+  HIP::AdamWRates rates;
+  AdamW(HIP& dev, std::vector<Buffer> params, const HIP::AdamWRates& r, bool eight = false, uint64_t seed = 0x51CED)
+      : rates(r), dev_(&dev), params_(std::move(params)), counter_(dev.alloc(2, true)), seed_(seed) {
+    for (const Buffer& p : params_) {
+      m_.push_back(dev.alloc(eight ? (p.len + 3) / 4 : p.len, true));
+      v_.push_back(dev.alloc(eight ? (p.len + 3) / 4 : p.len, true));
+      if (eight) scales_.push_back(dev.alloc(2 * ((p.len + 255) / 256), true));
+    }
+  }
+  ~AdamW() {
+    try {
+      for (const std::vector<Buffer>* set : {&m_, &v_, &scales_})
+        for (const Buffer& b : *set) dev_->release(b.id);
+      dev_->release(counter_.id);
+    } catch (const std::exception&) {  // (a device that is recording frees nothing; its buffers go with it)
+    }
+  }
+  AdamW(const AdamW&) = delete;
+  AdamW& operator=(const AdamW&) = delete;
+  void step() { dev_->adamw_step(params_, m_, v_, scales_, counter_, rates, seed_); }
+  HIP& device() const { return *dev_; }
+
+ private:
+  HIP* dev_;
+  std::vector<Buffer> params_, m_, v_, scales_;
+  Buffer counter_;
+  uint64_t seed_;
+};
+
 struct MlpResult {
   double seconds = 0.0;  // wall time of the timed steps, device idle on both sides
   size_t graph_nodes = 0;  // kernels per recorded step (MLP_GRAPH only)
@@ -59,6 +93,8 @@ enum MlpMode {
   MLP_FUSED = 1,  // Linear (+ReLU) forward as one kernel, ReLU gradient inside the next layer's input-gradient GEMM
   MLP_GRAPH = 2,  // step 0 runs eagerly, step 1 is recorded, every later step replays the recording
   MLP_FUSED_LOSS = 4,  // the loss chain (MSE, or softmax + cross-entropy) as one forward and one backward kernel
+  MLP_ADAMW = 16,      // AdamW instead of SGD, with its moments in f32 ...
+  MLP_ADAMW8 = 32,     // ... or in 8 bits
   MLP_WHOLE_STEP = 8   // kind 0 with at most 64 hidden units: the whole step as two launches (HIP::mlp3_mse_step)
 };
 
@@ -84,6 +120,14 @@ inline MlpResult mlp_train(HIP& dev, int kind, size_t batch, size_t d_in, size_t
   Matrix c(dev.from(&inv, 1), 1, 1);
   c.no_grad();
   SGD sgd{lr};
+  std::unique_ptr<AdamW> adamw;
+  if (mode & (MLP_ADAMW | MLP_ADAMW8)) {
+    if (mode & MLP_WHOLE_STEP) throw Error("the whole-step kernels train by SGD only");
+    HIP::AdamWRates rates;
+    rates.lr = lr;
+    adamw.reset(new AdamW(dev, {lin1.weights.data, lin1.bias.data, lin2.weights.data, lin2.bias.data, lin3.weights.data, lin3.bias.data}, rates,
+                          (mode & MLP_ADAMW8) != 0));
+  }
   // loss pieces of kind 1 live outside the cache: they are not tape outputs
   Buffer loss_rows = kind == 1 ? dev.alloc(batch, true) : Buffer();
   Buffer seed = kind == 1 ? dev.alloc(n_out, true) : Buffer();
@@ -131,7 +175,9 @@ inline MlpResult mlp_train(HIP& dev, int kind, size_t batch, size_t d_in, size_t
       check(slhip_cce_grad(dev.ctx(), batch, d_out, p.data.ptr, y.data.ptr, seed.ptr), "slhip_cce_grad");
       p.data.backward_with(seed);
     }
-    if (fused) {
+    if (adamw) {
+      adamw->step();
+    } else if (fused) {
       sgd.step(dev, {&lin1, &lin2, &lin3});
     } else {
       sgd.step(dev, lin1);

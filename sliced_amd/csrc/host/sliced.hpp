@@ -668,6 +668,57 @@ class HIP {
     return out;
   }
 
+  // Group norm with an activation over samples x positions x channels (slhip_group_norm; no counterpart in the
+  // reference).  weight and bias (channels each) may be empty buffers: ones and zeros.
+  Buffer group_norm(size_t samples, size_t positions, size_t channels, size_t groups, const Buffer& x, const Buffer& weight = Buffer(),
+                    const Buffer& bias = Buffer(), int act = SLHIP_ACT_NONE, float eps = 1e-5f) {
+    expect(x, samples * positions * channels, "group_norm x");
+    if (weight.valid()) { expect(weight, channels, "group_norm weight"); used(weight); }
+    if (bias.valid()) { expect(bias, channels, "group_norm bias"); used(bias); }
+    used(x);
+    Buffer mean = retrieve(samples * groups), rstd = retrieve(samples * groups), out = retrieve(x.len);
+    check(slhip_group_norm(ctx_, samples, positions, channels, groups, act, eps, x.ptr, weight.ptr, bias.ptr, mean.ptr, rstd.ptr, out.ptr),
+          "slhip_group_norm");
+    const uint64_t xi = x.id, wi = weight.id, bi = bias.id, mi = mean.id, ri = rstd.id, oi = out.id;
+    add_grad_fn([=] {
+      Buffer xb = lookup(xi), w = wi ? lookup(wi) : Buffer(), b = bi ? lookup(bi) : Buffer(), o = lookup(oi);
+      const float *mp = lookup(mi).ptr, *rp = lookup(ri).ptr, *og = grad(o).ptr;
+      into_grads({xb, w, b}, [&](float* const* g, float beta) {
+        check(slhip_group_norm_grad(ctx_, samples, positions, channels, groups, act, xb.ptr, w.ptr, b.ptr, mp, rp, g[0], g[1], g[2], og, beta),
+              "slhip_group_norm_grad");
+      });
+    });
+    return out;
+  }
+
+  // The gated linear recurrence over batch x steps x channels (slhip_gated_scan; no counterpart in the reference): the
+  // states of all steps.  h0 (batch x channels) may be an empty buffer: zeros.
+  Buffer gated_scan(int mode, size_t batch, size_t steps, size_t channels, const Buffer& gate, const Buffer& x, const Buffer& h0 = Buffer()) {
+    expect(gate, batch * steps * channels, "gated_scan gate"); expect(x, batch * steps * channels, "gated_scan x");
+    if (h0.valid()) { expect(h0, batch * channels, "gated_scan h0"); used(h0); }
+    used(gate, x);
+    Buffer out = retrieve(x.len);
+    check(slhip_gated_scan(ctx_, mode, batch, steps, channels, gate.ptr, x.ptr, h0.ptr, out.ptr, nullptr), "slhip_gated_scan");
+    const uint64_t gi = gate.id, xi = x.id, hi = h0.id, oi = out.id;
+    add_grad_fn([=] {
+      Buffer gb = lookup(gi), xb = lookup(xi), hb = hi ? lookup(hi) : Buffer(), o = lookup(oi);
+      const float* og = grad(o).ptr;
+      into_grads({gb, xb, hb}, [&](float* const* g, float beta) {
+        check(slhip_gated_scan_grad(ctx_, mode, batch, steps, channels, gb.ptr, xb.ptr, hb.ptr, o.ptr, g[0], g[1], g[2], og, nullptr, beta),
+              "slhip_gated_scan_grad");
+      });
+    });
+    return out;
+  }
+  // One step of it for a serving loop: `state` (batch x channels) becomes the next state, in place.  Not on the tape.
+  void gated_scan_step(int mode, size_t batch, size_t channels, const Buffer& gate, const Buffer& x, const Buffer& state) {
+    expect(gate, batch * channels, "gated_scan_step gate"); expect(x, batch * channels, "gated_scan_step x");
+    expect(state, batch * channels, "gated_scan_step state");
+    if (state.id == gate.id || state.id == x.id) throw Error("gated_scan_step: the state is one of the inputs");
+    ready(gate); ready(x); ready(state);
+    check(slhip_gated_scan(ctx_, mode, batch, 1, channels, gate.ptr, x.ptr, state.ptr, state.ptr, nullptr), "slhip_gated_scan");
+  }
+
   // Reductions with gradients: SumColsMayGrad (src/ops.rs:592-611), SumRows (forward + the slice
   // gradient; the reference's own wrapper is `unimplemented!()`, src/ops.rs:553-567),
   // MaxCols/MaxRows (:471-491, :515-534), MeanCols/MeanRows (:635-651, :675-684).
@@ -749,6 +800,42 @@ class HIP {
     ready(out);
     check(slhip_mean(ctx_, x.len, x.ptr, out.ptr), "slhip_mean");
   }
+  // One AdamW step of a whole parameter list (slhip_adamw_step_multi): moments of the parameters' lengths, or, with `scales`,
+  // 8-bit ones (slhip_adamw8_step_multi: a quarter of the length, in whole floats, and two scales a started block of 256).
+  // `counter` (two floats, read as one 64-bit count) is advanced on the device, so that a recorded step counts on.
+  struct AdamWRates {
+    float lr = 1e-3f, beta1 = 0.9f, beta2 = 0.999f, eps = 1e-8f, weight_decay = 0.01f;
+  };
+  void adamw_step(const std::vector<Buffer>& params, const std::vector<Buffer>& m, const std::vector<Buffer>& v,
+                  const std::vector<Buffer>& scales, const Buffer& counter, const AdamWRates& r, uint64_t seed = 0x51CED) {
+    const size_t count = params.size();
+    const bool eight = !scales.empty();
+    if (m.size() != count || v.size() != count || (eight && scales.size() != count)) throw Error("adamw_step: as many moments as parameters expected");
+    expect(counter, 2, "adamw_step counter");
+    run();
+    std::vector<float*> p, mp, vp, sp;
+    std::vector<const float*> g;
+    std::vector<size_t> n;
+    for (size_t i = 0; i < count; ++i) {
+      const size_t len = params[i].len, held = eight ? (len + 3) / 4 : len;
+      expect(m[i], held, "adamw_step m"); expect(v[i], held, "adamw_step v");
+      if (eight) { expect(scales[i], 2 * ((len + 255) / 256), "adamw_step scales"); sp.push_back(scales[i].ptr); }
+      ready(params[i]);
+      p.push_back(params[i].ptr);
+      g.push_back(grad(params[i]).ptr);
+      mp.push_back(m[i].ptr);
+      vp.push_back(v[i].ptr);
+      n.push_back(len);
+    }
+    if (eight)
+      check(slhip_adamw8_step_multi(ctx_, count, p.data(), g.data(), (void* const*)mp.data(), (void* const*)vp.data(), sp.data(), n.data(), r.lr,
+                                    r.beta1, r.beta2, r.eps, r.weight_decay, 0, (uint64_t*)counter.ptr, seed),
+            "slhip_adamw8_step_multi");
+    else
+      check(slhip_adamw_step_multi(ctx_, count, p.data(), g.data(), mp.data(), vp.data(), n.data(), r.lr, r.beta1, r.beta2, r.eps,
+                                   r.weight_decay, 0, (uint64_t*)counter.ptr),
+            "slhip_adamw_step_multi");
+  }
   void copy(const Buffer& src, size_t src_off, const Buffer& dst, size_t dst_off, size_t n) {
     if (src_off + n > src.len || dst_off + n > dst.len) throw Error("copy: range outside the buffer");
     ready(src);
@@ -807,6 +894,31 @@ class HIP {
   }
 
  private:
+  // The gradients of an op whose kernel writes them beta * old + new: f(pointers, beta) for the buffers that want one (null
+  // for the others).  Where all of them are known to hold zeros - not written since zero_grad() marked them, or never -
+  // they are overwritten instead of read and added to.  A buffer that the op reads twice gets its terms one after the other.
+  template <class F>
+  void into_grads(const std::vector<Buffer>& of, F&& f) {
+    std::vector<size_t> want;
+    bool zeros = true, twice = false;
+    for (size_t i = 0; i < of.size(); ++i) {
+      if (!of[i].valid() || !of[i].requires_grad) continue;
+      for (size_t j : want) twice = twice || of[j].id == of[i].id;
+      want.push_back(i);
+      auto it = grads_.find(of[i].id);
+      zeros = zeros && (it == grads_.end() || stale_.count(it->second.id) != 0);
+    }
+    if (want.empty()) return;
+    zeros = zeros && !twice;
+    std::vector<float*> g(of.size(), nullptr);
+    for (size_t i : want) {
+      g[i] = grad_out(of[i], zeros).ptr;
+      if (!twice) continue;
+      f(g.data(), 1.0f);
+      g[i] = nullptr;
+    }
+    if (!twice) f(g.data(), zeros ? 0.0f : 1.0f);
+  }
   // Every op's forward reports the buffers it reads.  What is counted: the consumers of a fused
   // Linear's ReLU output, because GradPolicy::fuse_relu_grad may skip that output's own gradient
   // only while exactly one op (the next fused Linear) reads it.
@@ -1152,6 +1264,16 @@ class Matrix {
   // carries its true shape.
   Matrix max_rows() const { return Matrix(device().reduce(HIP::MAX_ROWS, rows, cols, data), 1, cols); }
   Matrix max_cols() const { return Matrix(device().reduce(HIP::MAX_COLS, rows, cols, data), rows, 1); }
+  // Every row a position of samples of `positions` rows each, the columns in `groups` runs (slhip_group_norm).
+  Matrix group_norm(size_t groups, const Matrix& weight, const Matrix& bias, int act = SLHIP_ACT_NONE, size_t positions = 1) const {
+    if (positions == 0 || rows % positions != 0) throw Error("group_norm: rows are not whole samples");
+    return Matrix(device().group_norm(rows / positions, positions, cols, groups, data, weight.data, bias.data, act), rows, cols);
+  }
+  // The rows as `batch` sequences of rows / batch steps each (slhip_gated_scan).
+  Matrix gated_scan(int mode, size_t batch, const Matrix& gate) const {
+    if (batch == 0 || rows % batch != 0) throw Error("gated_scan: rows are not whole sequences");
+    return Matrix(device().gated_scan(mode, batch, rows / batch, cols, gate.data, data), rows, cols);
+  }
   Matrix as_dims(size_t r, size_t c) const { return Matrix(data, r, c); }                                       // :383-390
 };
 

@@ -24,6 +24,8 @@ LIB_PATH = os.path.join(HERE, "libsliced_host.so")
 ADD, SUB, MUL, DIV = 0, 1, 2, 3
 SQUARE, POW, RELU, EXP, CLIP, NEG_LN, SCALE, NEG_DIV, TANH, SIGMOID = range(10)
 SUM_ROWS, SUM_COLS, MAX_ROWS, MAX_COLS, MEAN_ROWS, MEAN_COLS = range(6)
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = range(4)
+SCAN_LINEAR, SCAN_SIGMOID = 0, 1
 
 _h = None
 
@@ -265,6 +267,22 @@ class HIP:
     def softmax(self, samples, features, x):
         return self._out(lib().slh_softmax, _sz(samples), _sz(features), _u64(x.id))
 
+    def group_norm(self, samples, positions, channels, groups, x, weight=None, bias=None, act=ACT_NONE, eps=1e-5):
+        return self._out(lib().slh_group_norm, _sz(samples), _sz(positions), _sz(channels), _sz(groups), _u64(x.id),
+                         _u64(weight.id if weight else 0), _u64(bias.id if bias else 0), int(act), _f(eps))
+
+    def gated_scan(self, mode, batch, steps, channels, gate, x, h0=None):
+        return self._out(lib().slh_gated_scan, int(mode), _sz(batch), _sz(steps), _sz(channels), _u64(gate.id), _u64(x.id),
+                         _u64(h0.id if h0 else 0))
+
+    def gated_scan_step(self, mode, batch, channels, gate, x, state):
+        """One token of a serving loop: `state` becomes the next state, in place."""
+        _ck(lib().slh_gated_scan_step(self.h, int(mode), _sz(batch), _sz(channels), _u64(gate.id), _u64(x.id), _u64(state.id)))
+
+    def adamw(self, params, lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8, weight_decay=0.01, eight=False, seed=rng.DEFAULT_SEED):
+        """An AdamW optimiser over a list of buffers, its moments in f32 or (eight) in 8 bits."""
+        return AdamW(self, params, lr, beta1, beta2, eps, weight_decay, eight, seed)
+
     def _red(self, kind, cols, x, rows=None):
         rows = len(x) // cols if rows is None else rows
         return self._out(lib().slh_reduce, int(kind), _sz(rows), _sz(cols), _u64(x.id))
@@ -296,6 +314,24 @@ class HIP:
         _ck(lib().slh_sgd_step(self.h, _u64(p.id), _f(lr)))
 
 
+class AdamW:
+    """Handle of a device's AdamW optimiser; close it before the device."""
+
+    def __init__(self, dev, params, lr, beta1, beta2, eps, weight_decay, eight, seed):
+        self.h = C.c_void_p()
+        ids = (_u64 * len(params))(*[p.id for p in params])
+        _ck(lib().slh_adamw_new(dev.h, _sz(len(params)), ids, _f(lr), _f(beta1), _f(beta2), _f(eps), _f(weight_decay), int(bool(eight)),
+                                _u64(seed), C.byref(self.h)))
+
+    def step(self):
+        _ck(lib().slh_adamw_step(self.h))
+
+    def close(self):
+        if self.h:
+            _ck(lib().slh_adamw_free(self.h))
+            self.h = None
+
+
 # ---------------------------------------------------------------------------- training loops
 def mlp_init(kind, d_in, d_h, d_out, seed=rng.DEFAULT_SEED):
     """Seeded parameters: U(+-1/sqrt(fan_in)) for the sine fit, Kaiming-uniform U(+-sqrt(6/fan_in))
@@ -321,10 +357,11 @@ def mlp_data(kind, batch, d_in, d_out, seed=rng.DEFAULT_SEED):
 
 
 def mlp_train(kind, batch, d_in, d_h, d_out, x, target, params, lr, steps, warmup=0, fused=False, ordinal=0,
-              graph=False, info=None, fused_loss=False, whole_step=False):
+              graph=False, info=None, fused_loss=False, whole_step=False, optimizer="sgd"):
     """Runs the C++ training loop on the GPU.  params (six float32 arrays) are updated in place.
     graph=True records one step as a HIP graph and replays it (losses are read once at the end).
     whole_step=True (the MSE loop with at most 64 hidden units) runs every step as two launches.
+    optimizer: "sgd", "adamw" or "adamw8" (AdamW with 8-bit moments).
     Returns (losses[steps], seconds for the timed steps); info, a dict, receives graph_nodes."""
     losses = np.zeros(steps, np.float32)
     secs = C.c_double()
@@ -333,7 +370,8 @@ def mlp_train(kind, batch, d_in, d_h, d_out, x, target, params, lr, steps, warmu
     x = np.ascontiguousarray(x, np.float32)
     target = np.ascontiguousarray(target, np.float32)
     _ck(lib().slh_mlp_train(ordinal, int(kind), _sz(batch), _sz(d_in), _sz(d_h), _sz(d_out), p(x), p(target),
-                            *[p(a) for a in params], _f(lr), _sz(steps), _sz(warmup), int(bool(fused)) | (2 if graph else 0) | (4 if fused_loss else 0) | (8 if whole_step else 0),
+                            *[p(a) for a in params], _f(lr), _sz(steps), _sz(warmup), int(bool(fused)) | (2 if graph else 0) | (4 if fused_loss else 0) | (8 if whole_step else 0)
+                            | {"sgd": 0, "adamw": 16, "adamw8": 32}[optimizer],
                             p(losses), C.byref(secs), C.byref(nodes)))
     if info is not None:
         info["graph_nodes"] = nodes.value
