@@ -250,13 +250,14 @@ int32_t slhip_softmax_grad(slhip_ctx* ctx, size_t samples, size_t features, floa
  *     mean, rstd = 1/sqrt(var + eps);  u = (x − mean)·rstd·weight[c] + bias[c];  out = act(u)
  * groups = 1 and positions = 1 is a layer norm of every row.  weight and bias (channels each) may be
  * NULL (ones, zeros).  mean and rstd (samples × groups each) receive what the backward pass needs and
- * may be NULL.  out may alias x.
+ * may be NULL.  out may be x itself; any other overlap with an input is refused (SLHIP_EALIAS).  At most 2^31 − 1
+ * channels.
  * slhip_group_norm_grad, with g = out_grad ⊙ act'(u), hat = (x − mean)·rstd, gx = g·weight, < > a mean over the
  * sample's group:
  *     x_grad      = beta·x_grad + rstd·(gx − <gx> − hat·<gx·hat>)
  *     weight_grad = beta·weight_grad + Σ g·hat      bias_grad = beta·bias_grad + Σ g
  * beta 0 = SET, 1 = accumulate.  x_grad, weight_grad and bias_grad may each be NULL (skipped); x_grad may
- * alias out_grad.  Every sum has a fixed order.  SLHIP_ACT_GELU is x·Φ(x) with the error function, relu'
+ * be out_grad itself; any other overlap is refused.  Every sum has a fixed order.  SLHIP_ACT_GELU is x·Φ(x) with the error function, relu'
  * is (u >= 0) as everywhere here. */
 enum { SLHIP_ACT_NONE = 0, SLHIP_ACT_RELU = 1, SLHIP_ACT_SILU = 2, SLHIP_ACT_GELU = 3 };
 int32_t slhip_group_norm(slhip_ctx* ctx, size_t samples, size_t positions, size_t channels, size_t groups, int32_t act,
@@ -272,8 +273,8 @@ int32_t slhip_group_norm_grad(slhip_ctx* ctx, size_t samples, size_t positions, 
  *     SLHIP_SCAN_LINEAR   h_t = gate_t·h_{t−1} + x_t
  *     SLHIP_SCAN_SIGMOID  h_t = s·h_{t−1} + (1 − s)·x_t,  s = 1/(1 + exp(−gate_t))
  * h_{−1} is h0 (batch × channels; NULL: zeros).  h_last (may be NULL) receives h_{steps−1}, the h0 of a call that
- * goes on from here - steps = 1 is one token of a serving loop - and may be h0 itself.  h may alias x
- * or gate when it is the same array.
+ * goes on from here - steps = 1 is one token of a serving loop - and may be h0 itself.  h may be x
+ * or gate itself and, with steps = 1, h0 itself; any other overlap is refused (SLHIP_EALIAS).
  * Long sequences are cut into runs that are joined by their products of gates, in a fixed order.  For
  * SLHIP_SCAN_LINEAR a product of gates over a run of steps has to be representable: gates of magnitude
  * up to one always are.
@@ -281,7 +282,7 @@ int32_t slhip_group_norm_grad(slhip_ctx* ctx, size_t samples, size_t positions, 
  * d_t = h_grad_t + a_{t+1}·d_{t+1} (a = gate or s; d_{steps-1} also takes h_last_grad):
  *     LINEAR   gate_grad = d·h_{t−1}                   x_grad = d
  *     SIGMOID  gate_grad = d·(h_{t−1} − x)·s·(1 − s)      x_grad = d·(1 − s)         h0_grad = a_0·d_0
- * each beta·(old value) + that; each may be NULL (skipped), and none may overlap an input.  x may be NULL
+ * each beta·(old value) + that; each may be NULL (skipped), and none may overlap an input or another.  x may be NULL
  * for SLHIP_SCAN_LINEAR. */
 enum { SLHIP_SCAN_LINEAR = 0, SLHIP_SCAN_SIGMOID = 1 };
 int32_t slhip_gated_scan(slhip_ctx* ctx, int32_t mode, size_t batch, size_t steps, size_t channels, const float* gate,
@@ -390,8 +391,8 @@ int32_t slhip_sgd_step_multi(slhip_ctx* ctx, size_t count, float* const* params,
  * as zeros.  t is `step`, counted from 1; or, with step = 0, the counter that step_dev (a device
  * pointer, 8-byte aligned, starting at zero) names, which the call advances by one first: that is the
  * form for recorded steps, whose replays must not repeat one t (one more small launch, which leaves
- * what it computes in the workspace).  No two tensors may overlap (SLHIP_EALIAS), nor a gradient any
- * array that is written.  beta1 and beta2 lie in [0, 1), eps >= 0.
+ * what it computes in the workspace).  No array that the call writes may overlap any other
+ * (SLHIP_EALIAS); count is at most 16384.  beta1 and beta2 lie in [0, 1), eps >= 0.
  * slhip_adamw8_step_multi keeps the moments in 8 bits: m8[i] holds lens[i] OCP E4M3 values, v8[i] lens[i]
  * OCP E5M2 values (both 4-byte aligned), and scales[i] two floats, m's and v's, for every started block
  * of 256 elements; a moment is its 8-bit value times its block's scale, a power of two.  All start as

@@ -22,7 +22,9 @@
 // before they are rounded.
 #include "common.hpp"
 
+#include <algorithm>
 #include <cmath>
+#include <new>
 
 namespace slhip {
 
@@ -30,6 +32,7 @@ constexpr int ADAMW_TENSORS = 64;   // of one launch: a lane each in the search 
 constexpr int ADAMW_BLOCK = 256;    // elements of a scale: a wave's 64 lanes hold four each
 constexpr int ADAMW_ROWS = 2;       // blocks of 256 elements a wave takes
 constexpr size_t ADAMW_TILE = (size_t)4 * ADAMW_ROWS * ADAMW_BLOCK;  // elements of a workgroup of four waves
+constexpr size_t ADAMW_LONGEST = MAX_GRID / ADAMW_TENSORS * ADAMW_TILE;  // elements of a tensor: 64 of them fit a launch
 
 // What depends on the number of the step: passed by value, or left in the workspace by adamw_advance_kernel.
 struct AdamwStep {
@@ -280,14 +283,50 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Adamw8Args a) {
   }
 }
 
-// Two of the first `m` arrays overlap (bytes[i] long): the workgroups of one launch would race on them.
-static bool adamw_overlap(const void* const* at, const size_t* lens, size_t unit, size_t m) {
-  for (size_t i = 1; i < m; ++i)
-    for (size_t j = 0; j < i; ++j) {
-      const uintptr_t a = (uintptr_t)at[i], b = (uintptr_t)at[j];
-      if (a < b + lens[j] * unit && b < a + lens[i] * unit) return true;
+// The arrays of a call, in the order of their addresses: 2^47 of those and 2^17 arrays make one 64-bit key, whose sorting
+// takes 2 us for 64 tensors.
+constexpr size_t ADAMW_MOST = 16384;  // tensors of a call
+static_assert(5 * ADAMW_MOST <= (size_t(1) << 17), "arrays of a call");
+
+// Whether an array that the call writes shares memory with any other.  `arrays` kinds of `count` pointers each; bytes(kind, i)
+// is an array's length, `read_only` the kind that is not written.
+template <class F>
+static int32_t adamw_overlap(const char* who, const void* const* const* arrays, int kinds, int read_only, size_t count, F&& bytes) {
+  uint64_t few[5 * ADAMW_TENSORS];
+  uint64_t* keys = few;
+  const size_t n = count * (size_t)kinds;
+  if (count > ADAMW_TENSORS && !(keys = new (std::nothrow) uint64_t[n])) {
+    set_error("%s: out of host memory", who);
+    return SLHIP_EINVAL;
+  }
+  size_t k = 0;
+  uint64_t high = 0;
+  for (int kind = 0; kind < kinds; ++kind)
+    for (size_t i = 0; i < count; ++i, ++k) {
+      const uint64_t at = (uint64_t)(uintptr_t)arrays[kind][i];
+      high |= at >> 47;
+      keys[k] = at << 17 | k;
     }
-  return false;
+  std::sort(keys, keys + n);
+  uint64_t any = 0, written = 0;  // where the arrays so far end, and those of them that are written
+  bool shared = false;
+  for (size_t i = 0; i < n; ++i) {
+    const uint64_t at = keys[i] >> 17, which = keys[i] & ((1u << 17) - 1);
+    const int kind = (int)(which / count);
+    const uint64_t end = at + bytes(kind, (size_t)(which % count));
+    const bool writes = kind != read_only;
+    shared = shared || at < (writes ? any : written);
+    if (any < end) any = end;
+    if (writes && written < end) written = end;
+  }
+  if (keys != few) delete[] keys;
+  if (high) {
+    set_error("%s: not a device address", who);
+    return SLHIP_EINVAL;
+  }
+  if (!shared) return SLHIP_OK;
+  set_error("%s: two tensors overlap", who);
+  return SLHIP_EALIAS;
 }
 
 // Checks what both forms share and fills in the rates; the step of the call comes from the host or, where
@@ -324,7 +363,7 @@ static int32_t adamw_begin(slhip_ctx* ctx, const char* who, float lr, float beta
   return post_launch();
 }
 
-// Numbers the workgroups of tensors first .. first + m and returns how many there are (0: too many for one launch).
+// Numbers the workgroups of tensors first .. first + m and returns how many there are.
 template <class Args>
 static size_t adamw_number(Args& a, const size_t* lens, size_t m) {
   size_t blocks = 0;
@@ -332,7 +371,6 @@ static size_t adamw_number(Args& a, const size_t* lens, size_t m) {
     a.n[i] = i < m ? lens[i] : 0;
     a.first[i] = i < m ? (unsigned)blocks : ~0u;
     if (i < m) blocks += (lens[i] + ADAMW_TILE - 1) / ADAMW_TILE;
-    if (blocks > MAX_GRID) return 0;
   }
   return blocks;
 }
@@ -345,22 +383,17 @@ SLHIP_API int32_t slhip_adamw_step_multi(slhip_ctx* ctx, size_t count, float* co
                                          float* const* v, const size_t* lens, float lr, float beta1, float beta2, float eps,
                                          float weight_decay, uint64_t step, uint64_t* step_dev) {
   SLHIP_REQUIRE(ctx && params && grads && m && v && lens, "null argument");
-  SLHIP_REQUIRE(count > 0, "no tensors");
+  SLHIP_REQUIRE(count > 0 && count <= ADAMW_MOST, "no tensors, or too many");
   for (size_t i = 0; i < count; ++i) {
     SLHIP_REQUIRE(params[i] && grads[i] && m[i] && v[i] && lens[i] > 0, "null or empty tensor");
-    SLHIP_REQUIRE(lens[i] <= SIZE_MAX / 8, "tensor too long");
+    SLHIP_REQUIRE(lens[i] <= ADAMW_LONGEST, "tensor too long");
   }
-  for (size_t at = 0; at < count; at += ADAMW_TENSORS) {
-    const size_t k = count - at < (size_t)ADAMW_TENSORS ? count - at : (size_t)ADAMW_TENSORS;
-    if (adamw_overlap((const void* const*)(params + at), lens + at, 4, k) || adamw_overlap((const void* const*)(m + at), lens + at, 4, k) ||
-        adamw_overlap((const void* const*)(v + at), lens + at, 4, k)) {
-      set_error("slhip_adamw_step_multi: two tensors overlap");
-      return SLHIP_EALIAS;
-    }
-  }
+  const void* const* const arrays[] = {(const void* const*)params, (const void* const*)grads, (const void* const*)m, (const void* const*)v};
+  int32_t rc = adamw_overlap("slhip_adamw_step_multi", arrays, 4, 1, count, [&](int, size_t i) { return lens[i] * sizeof(float); });
+  if (rc) return rc;
   SLHIP_ON_DEVICE(ctx);
   AdamwArgs a;
-  int32_t rc = adamw_begin(ctx, "slhip_adamw_step_multi", lr, beta1, beta2, eps, weight_decay, step, step_dev, 0, &a.r, &a.step, &a.step_dev);
+  rc = adamw_begin(ctx, "slhip_adamw_step_multi", lr, beta1, beta2, eps, weight_decay, step, step_dev, 0, &a.r, &a.step, &a.step_dev);
   if (rc) return rc;
   for (size_t at = 0; at < count; at += ADAMW_TENSORS) {
     const size_t k = count - at < (size_t)ADAMW_TENSORS ? count - at : (size_t)ADAMW_TENSORS;
@@ -369,7 +402,6 @@ SLHIP_API int32_t slhip_adamw_step_multi(slhip_ctx* ctx, size_t count, float* co
       a.p[i] = params[j]; a.g[i] = grads[j]; a.m[i] = m[j]; a.v[i] = v[j];
     }
     const size_t blocks = adamw_number(a, lens + at, k);
-    SLHIP_REQUIRE(blocks > 0, "tensors too long for one launch");
     hipLaunchKernelGGL(adamw_kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, a);
     rc = post_launch();
     if (rc) return rc;
@@ -381,30 +413,21 @@ SLHIP_API int32_t slhip_adamw8_step_multi(slhip_ctx* ctx, size_t count, float* c
                                           void* const* v8, float* const* scales, const size_t* lens, float lr, float beta1, float beta2,
                                           float eps, float weight_decay, uint64_t step, uint64_t* step_dev, uint64_t seed) {
   SLHIP_REQUIRE(ctx && params && grads && m8 && v8 && scales && lens, "null argument");
-  SLHIP_REQUIRE(count > 0 && count <= 0xffffffffu, "no tensors, or too many");
+  SLHIP_REQUIRE(count > 0 && count <= ADAMW_MOST, "no tensors, or too many");
   for (size_t i = 0; i < count; ++i) {
     SLHIP_REQUIRE(params[i] && grads[i] && m8[i] && v8[i] && scales[i] && lens[i] > 0, "null or empty tensor");
-    SLHIP_REQUIRE(lens[i] <= SIZE_MAX / 8, "tensor too long");
+    SLHIP_REQUIRE(lens[i] <= ADAMW_LONGEST, "tensor too long");
     SLHIP_REQUIRE((((uintptr_t)m8[i] | (uintptr_t)v8[i]) & 3) == 0, "8-bit moments must be 4-byte aligned");
   }
-  for (size_t at = 0; at < count; at += ADAMW_TENSORS) {
-    const size_t k = count - at < (size_t)ADAMW_TENSORS ? count - at : (size_t)ADAMW_TENSORS;
-    if (adamw_overlap((const void* const*)(params + at), lens + at, 4, k) || adamw_overlap((const void* const*)(m8 + at), lens + at, 1, k) ||
-        adamw_overlap((const void* const*)(v8 + at), lens + at, 1, k)) {
-      set_error("slhip_adamw8_step_multi: two tensors overlap");
-      return SLHIP_EALIAS;
-    }
-    for (size_t i = at + 1; i < at + k; ++i)
-      for (size_t j = at; j < i; ++j)
-        if ((uintptr_t)scales[i] < (uintptr_t)scales[j] + 8 * ((lens[j] + ADAMW_BLOCK - 1) / ADAMW_BLOCK) &&
-            (uintptr_t)scales[j] < (uintptr_t)scales[i] + 8 * ((lens[i] + ADAMW_BLOCK - 1) / ADAMW_BLOCK)) {
-          set_error("slhip_adamw8_step_multi: two tensors' scales overlap");
-          return SLHIP_EALIAS;
-        }
-  }
+  const void* const* const arrays[] = {(const void* const*)params, (const void* const*)grads, (const void* const*)m8, (const void* const*)v8,
+                                       (const void* const*)scales};
+  int32_t rc = adamw_overlap("slhip_adamw8_step_multi", arrays, 5, 1, count, [&](int kind, size_t i) {
+    return kind < 2 ? lens[i] * sizeof(float) : kind < 4 ? lens[i] : (lens[i] + ADAMW_BLOCK - 1) / ADAMW_BLOCK * 2 * sizeof(float);
+  });
+  if (rc) return rc;
   SLHIP_ON_DEVICE(ctx);
   Adamw8Args a;
-  int32_t rc = adamw_begin(ctx, "slhip_adamw8_step_multi", lr, beta1, beta2, eps, weight_decay, step, step_dev, seed, &a.r, &a.step, &a.step_dev);
+  rc = adamw_begin(ctx, "slhip_adamw8_step_multi", lr, beta1, beta2, eps, weight_decay, step, step_dev, seed, &a.r, &a.step, &a.step_dev);
   if (rc) return rc;
   for (size_t at = 0; at < count; at += ADAMW_TENSORS) {
     const size_t k = count - at < (size_t)ADAMW_TENSORS ? count - at : (size_t)ADAMW_TENSORS;
@@ -414,7 +437,6 @@ SLHIP_API int32_t slhip_adamw8_step_multi(slhip_ctx* ctx, size_t count, float* c
     }
     a.ordinal = (unsigned)at;
     const size_t blocks = adamw_number(a, lens + at, k);
-    SLHIP_REQUIRE(blocks > 0, "tensors too long for one launch");
     hipLaunchKernelGGL(adamw8_kernel, dim3((unsigned)blocks), dim3(256), 0, ctx->stream, a);
     rc = post_launch();
     if (rc) return rc;

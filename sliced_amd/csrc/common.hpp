@@ -104,6 +104,13 @@ class OnDevice {
   slhip::OnDevice on_device_((ctx)->device);  \
   SLHIP_CHECK_HIP(on_device_.status())
 
+// A range of floats (none at a null pointer) and whether two of them share one.
+struct Range {
+  const float* at;
+  size_t n;
+};
+inline bool meet(const Range& a, const Range& b) { return a.at && b.at && a.at < b.at + b.n && b.at < a.at + a.n; }
+
 // rows*cols with overflow check; false on overflow or zero.
 inline bool checked_len(size_t rows, size_t cols, size_t* len) {
   if (rows == 0 || cols == 0) return false;
@@ -195,9 +202,8 @@ __device__ __forceinline__ void st1s(float* p, float v) { __builtin_nontemporal_
 
 // 1/(1 + exp(-z)) and 1/(1 + exp(z)), which add up to one, each to about two units in its last place at either end: with
 // e = exp(-|z|) nothing overflows, and the smaller of the two is e / (1 + e), not a difference.  The hardware's 2^x and
-// reciprocal with a correction each (the rounding of |z| log2(e) is put back as a factor 1 + lo ln 2; one Newton step),
-// since the library's exponential and the IEEE quotient take twice the instructions: the gated recurrence, where the
-// sigmoid is most of the arithmetic, is bound by it.
+// reciprocal with a correction each (the rounding of |z| log2(e) is put back as a factor 1 + lo ln 2; one Newton step):
+// half the instructions of the library's exponential and the IEEE quotient.
 __device__ __forceinline__ void sigmoid_pair(float z, float& s, float& rest) {
   float t = fabsf(z);
   t = t > 150.0f ? 150.0f : t;  // keeps NaN; e is zero from 104 on

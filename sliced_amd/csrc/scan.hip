@@ -584,6 +584,12 @@ SLHIP_API int32_t slhip_gated_scan(slhip_ctx* ctx, int32_t mode, size_t batch, s
   SLHIP_REQUIRE(ctx && gate && x && h, "null argument");
   SLHIP_REQUIRE(mode == SLHIP_SCAN_LINEAR || mode == SLHIP_SCAN_SIGMOID, "unknown mode");
   SLHIP_REQUIRE(checked_len(batch, channels, &state) && checked_len(state, steps, &len), "bad dims");
+  const Range out = {h, len}, end = {h_last, state};
+  if ((h != x && meet(out, {x, len})) || (h != gate && meet(out, {gate, len})) || (!(h == h0 && steps == 1) && meet(out, {h0, state})) ||
+      meet(end, out) || meet(end, {x, len}) || meet(end, {gate, len}) || (h_last != h0 && meet(end, {h0, state}))) {
+    set_error("slhip_gated_scan: an output overlaps an input, or the other one");
+    return SLHIP_EALIAS;
+  }
   SLHIP_ON_DEVICE(ctx);
   ScanArgs a = {};
   a.batch = batch; a.steps = steps; a.channels = channels;
@@ -599,6 +605,15 @@ SLHIP_API int32_t slhip_gated_scan_grad(slhip_ctx* ctx, int32_t mode, size_t bat
   SLHIP_REQUIRE(ctx && gate && h && h_grad && (x || mode == SLHIP_SCAN_LINEAR), "null argument");
   SLHIP_REQUIRE(checked_len(batch, channels, &state) && checked_len(state, steps, &len), "bad dims");
   if (!gate_grad && !x_grad && !h0_grad) return SLHIP_OK;
+  const Range outs[] = {{gate_grad, len}, {x_grad, len}, {h0_grad, state}};
+  const Range ins[] = {{gate, len}, {x, len}, {h, len}, {h_grad, len}, {h0, state}, {h_last_grad, state}};
+  bool shared = meet(outs[0], outs[1]) || meet(outs[0], outs[2]) || meet(outs[1], outs[2]);
+  for (const Range& o : outs)
+    for (const Range& i : ins) shared = shared || meet(o, i);
+  if (shared) {
+    set_error("slhip_gated_scan_grad: a gradient overlaps an input, or another one");
+    return SLHIP_EALIAS;
+  }
   SLHIP_ON_DEVICE(ctx);
   ScanArgs a = {};
   a.batch = batch; a.steps = steps; a.channels = channels;

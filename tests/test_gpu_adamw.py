@@ -382,6 +382,21 @@ def refused(lib, ctx):
         both(-4, arrays=ok[:k] + [two(at, at)] + ok[k + 1:])
         both(-4, arrays=ok[:k] + [two(at, at + 12)] + ok[k + 1:])
     assert e(ctx, 2, *ok, two(at + 512, at + 516), lens, *rates, 1, None, 0) == -4
+    both(-4, arrays=[ok[0], ok[0], ok[2], ok[3]])                       # gradients that are the parameters
+    both(-4, arrays=[ok[0], ok[1], ok[3], ok[3]])                       # one set of moments for both
+    both(-4, arrays=[ok[0], two(at + 128, at + 260), ok[2], ok[3]])     # a gradient that ends in a moment
+    both(-1, arrays=[ok[0], two(at + 128, at + 132), ok[2], ok[3]], rates=[nan] + rates[1:])  # gradients may (it is the rate that is refused)
+    assert e(ctx, 2, *ok, two(at + 512, at + 8), lens, *rates, 1, None, 0) == -4              # a scale inside a parameter
+    # one parameter twice, further apart than the tensors of a launch
+    many = [(C.c_void_p * 70)(*[at + 4 * (70 * k + i) for i in range(70)]) for k in range(5)]
+    ones = (C.c_size_t * 70)(*[1] * 70)
+    apart = [(C.c_void_p * 70)(*[at + 8 * (70 * k + i) for i in range(70)]) for k in range(5)]
+    assert f(ctx, 70, *many[:4], ones, nan, *rates[1:], 1, None) == -1
+    assert e(ctx, 70, *apart, ones, nan, *rates[1:], 1, None, 0) == -1
+    many[0][69], apart[0][69] = many[0][2], apart[0][2]
+    assert f(ctx, 70, *many[:4], ones, *rates, 1, None) == -4
+    assert e(ctx, 70, *apart, ones, *rates, 1, None, 0) == -4
+    both(-1, n=16385)
     assert e(ctx, 2, *ok[:2], two(at + 257, at + 320), ok[3], scales, lens, *rates, 1, None, 0) == -1
     assert e(ctx, 2, *ok, None, lens, *rates, 1, None, 0) == -1
 

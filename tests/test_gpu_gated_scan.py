@@ -229,6 +229,53 @@ def test_state_updated_in_place_over_long_sequences(hip, batch, steps, channels)
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("mode", [LINEAR, SIGMOID])
+@pytest.mark.parametrize("batch,steps,channels", [(3, 1, 37), (2, 5, 130), (2, 700, 33), (1, 5000, 67)])
+def test_outputs_over_inputs_equal_separate_ones(hip, batch, steps, channels, mode):
+    gate, x, h0 = data(mode, batch, steps, channels, tag=47)
+    want = hip.gated_scan(mode, batch, steps, channels, gate, x, h0)[0]
+    same = hip.gated_scan(mode, batch, steps, channels, gate, gate, h0)[0]
+    c = hip.ctx()
+    for over in range(3):
+        if over == 2 and steps > 1:
+            continue
+        g, v, s = c.array(gate), c.array(x), c.array(h0)
+        out = (g, v, s)[over]
+        c.call("slhip_gated_scan", mode, batch, steps, channels, g.ptr, v.ptr, s.ptr, out.ptr, None)
+        assert np.array_equal(out.numpy(), want), over
+        for b in (g, v, s):
+            b.free()
+    g, s = c.array(gate), c.array(h0)                 # gate, input and output in one
+    c.call("slhip_gated_scan", mode, batch, steps, channels, g.ptr, g.ptr, s.ptr, g.ptr, s.ptr)
+    assert np.array_equal(g.numpy(), same) and np.array_equal(s.numpy().reshape(batch, channels), same.reshape(batch, steps, channels)[:, -1])
+    g.free()
+    s.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("mode", [LINEAR, SIGMOID])
+def test_two_contexts_on_two_streams(hip, mode):
+    """A context of its own and one on a stream of torch's, both busy with split sequences at once: each has its own workspace."""
+    import torch
+    from sliced_amd.device import Context
+    batch, steps, channels = 1, 9000, 40
+    stream = torch.cuda.Stream()
+    one, two = Context(0), Context(0, stream=stream.cuda_stream)
+    sets = [data(mode, batch, steps, channels, tag=60 + 5 * k) for k in range(2)]
+    want = [hip.gated_scan(mode, batch, steps, channels, *s)[0] for s in sets]
+    bufs = [[c.array(a) for a in s] + [c.empty(s[0].size)] for c, s in zip((one, two), sets)]
+    for _ in range(10):
+        for c, b in zip((one, two), bufs):
+            c.call("slhip_gated_scan", mode, batch, steps, channels, b[0].ptr, b[1].ptr, b[2].ptr, b[3].ptr, None)
+    for c, b, w in zip((one, two), bufs, want):
+        c.sync()
+        assert np.array_equal(b[3].numpy(), w)
+    for c, b in zip((one, two), bufs):
+        for k in b:
+            k.free()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("steps", [50, 5000])
 def test_a_closed_gate_starts_a_sequence_anew(hip, steps):
     """gate 0 (linear) and -inf (sigmoid) forget what was before exactly - packed sequences; +inf keeps the state as it is."""
@@ -345,6 +392,20 @@ def refused(lib, ctx):
     assert grad(ctx, 0, 1, 1, 1, p, None, None, None, p, p, p, p, None, 0.0) == -1
     assert grad(ctx, 0, 1, 1, 1, p, None, None, p, p, p, p, None, None, 0.0) == -1
     assert grad(ctx, 0, 1, 1, 1, p, None, None, p, None, None, None, p, None, 0.0) == 0  # nothing asked for
+    # four floats each of gate, x and h, two of the states, and their gradients; outputs over anything else are refused
+    q = [p + 16 * k for k in range(9)]
+    for out in (q[0] + 4, q[1] - 4, q[2], q[2] + 4):
+        assert call(ctx, 0, 1, 2, 2, q[0], q[1], q[2], out, q[4]) == -4, out
+    for last in (q[0], q[1] + 12, q[2] + 4, q[3], q[3] + 8):
+        assert call(ctx, 0, 1, 2, 2, q[0], q[1], q[2], q[3], last) == -4, last
+    assert call(ctx, 0, 1, 1, 4, q[0], q[1], q[2], q[2], q[2]) == -4
+    ok = [q[0], q[1], q[2], q[3], q[4], q[5], q[6], q[7], q[8]]
+    for k in (4, 5, 6):
+        for other in range(9):
+            if other != k:
+                args = list(ok)
+                args[k] = ok[other]
+                assert grad(ctx, 1, 1, 2, 2, *args, 0.0) == -4, (k, other)
 
 
 def test_refusals_come_before_anything_touches_the_device():

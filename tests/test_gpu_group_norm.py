@@ -262,6 +262,42 @@ def test_float_aligned_operands_and_untouched_surroundings(hip, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(7, 1, 390, 13), (3, 1, 1001, 7), (2, 1, 9000, 1), (2, 9, 32, 4), (5, 333, 12, 12), (1, 5000, 16, 4), (2, 3, 2600, 1)])
+def test_outputs_over_inputs_equal_separate_ones(hip, shape):
+    x, w, b, dy = data(shape, SILU, tag=63)
+    out, mean, rstd = hip.group_norm(*shape, x, w, b, act=SILU)
+    want = [np.zeros(x.size, np.float32), np.zeros(shape[2], np.float32), np.zeros(shape[2], np.float32)]
+    hip.group_norm_grad(*shape, x, w, b, mean, rstd, dy, *want, act=SILU)
+    c = hip.ctx()
+    X, W, B, M, R, G = [c.array(a) for a in (x, w, b, mean, rstd, dy)]
+    GW, GB = c.empty(shape[2]), c.empty(shape[2])
+    c.call("slhip_group_norm_grad", *shape, SILU, X.ptr, W.ptr, B.ptr, M.ptr, R.ptr, G.ptr, GW.ptr, GB.ptr, G.ptr, 0.0)
+    for got, k in zip((G, GW, GB), want):
+        assert np.array_equal(got.numpy(), k)
+    c.call("slhip_group_norm", *shape, SILU, 1e-5, X.ptr, W.ptr, B.ptr, M.ptr, R.ptr, X.ptr)
+    for got, k in zip((X, M, R), (out, mean, rstd)):
+        assert np.array_equal(got.numpy(), k)
+    for k in (X, W, B, M, R, G, GW, GB):
+        k.free()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 200000, 4, 1), (1, 3000, 8, 2), (3, 1, 512, 1)])
+def test_one_value_far_from_the_rest(hip, shape):
+    """A group whose first value is 10^6 standard deviations of the rest away: it is nearly all of the variance, and the sums
+    of squares taken around it, or around any other value, must not lose the mean."""
+    x = rng.normal(int(np.prod(shape[:3])), 1.0, tag=67, seed=SEED).reshape(shape[:3]).astype(np.float32)
+    for n in range(shape[0]):
+        x[n, 0, ::shape[2] // shape[3]] = 1e6
+    (want, mean, rstd), (tol, tm, tr) = forward(shape, x, None, None, NONE, 1e-5)
+    got, m, r = hip.group_norm(*shape, x)
+    size = shape[1] * shape[2] // shape[3]
+    # the mean is off by a few roundings of the sums' largest terms, 1e6 / size, 1/sqrt(var) by some of itself
+    assert np.abs(m.reshape(mean.shape) - mean).max() <= 64 * U * 1e6 / min(size, 512)
+    assert np.abs(r.reshape(rstd.shape) / rstd - 1).max() <= 64 * U
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("shape", [(40, 1, 128, 4), (4, 700, 24, 2), (8, 16, 64, 8)])
 def test_recorded_calls_replay_like_the_eager_ones(hip, shape):
     c = hip.ctx()
@@ -311,6 +347,25 @@ def refused(lib, ctx):
         args[k] = None
         assert grad(ctx, 1, 1, 4, 2, 0, *args, 0.0) == -1, k
     assert grad(ctx, 1, 1, 4, 2, 0, p, p, p, p, p, None, None, None, p, 0.0) == 0  # nothing asked for
+    for bad in ((1, 1, 1 << 31, 1, 0), (1, 1, 1 << 33, 1 << 32, 0)):
+        assert call(ctx, *bad, 1e-5, p, None, None, None, None, p + (1 << 40)) == -1, bad
+        assert grad(ctx, *bad, p, None, None, p, p, p + (1 << 40), None, None, p, 0.0) == -1, bad
+    # x, weight, bias, mean, rstd, out: four floats each; an output over anything but x is refused
+    q = [p + 16 * k for k in range(9)]
+    for k in (3, 4, 5):
+        for other in range(6):
+            if other != k and (k, other) != (5, 0):
+                args = q[:6]
+                args[k] = q[other]
+                assert call(ctx, 2, 1, 2, 1, 0, 1e-5, *args) == -4, (k, other)
+    assert call(ctx, 2, 1, 2, 1, 0, 1e-5, *q[:5], q[0] + 4) == -4
+    for k in (5, 6, 7):
+        for other in range(9):
+            if other != k and (k, other) != (5, 8):
+                args = list(q)
+                args[k] = q[other]
+                assert grad(ctx, 2, 1, 2, 1, 0, *args, 0.0) == -4, (k, other)
+    assert grad(ctx, 2, 1, 2, 1, 0, *q[:5], q[8] + 4, q[6], q[7], q[8], 0.0) == -4
 
 
 def test_refusals_come_before_anything_touches_the_device():
