@@ -91,25 +91,22 @@ __device__ __forceinline__ NormVec<V> norm_param(const float* p, size_t c, float
   return r;
 }
 
-// The normal distribution's function and density at u, for x * Phi(x) and its slope.  erfc(x) is exp(-x^2), the density's
-// exponential too, times a polynomial without constant in 1/(1 + 0.325 x): the form of Abramowitz and Stegun's formula
+// What is left of a normal distribution beyond |u|, erfc(|u| / sqrt 2) / 2, and exp(-u^2 / 2), for x * Phi(x) and its slope.
+// erfc(x) is exp(-x^2) times a polynomial without constant in 1/(1 + 0.325 x): the form of Abramowitz and Stegun's formula
 // 7.1.26, three terms longer, its coefficients fitted here by reweighted least squares: 1.3e-8 off, and 2.6e-7 of itself
 // far out.  (The library's erff takes a branch each for small and large arguments, which both run in a wave; with it the
-// arithmetic, not HBM, bounded these kernels: 10 x 961 x 390 forward 17 us instead of 12.)
-__device__ __forceinline__ float norm_normal(float u, float& density) {
-  const float x = fabsf(u) * 0.70710678118654752f;
-  const float t = __builtin_amdgcn_rcpf(fmaf(0.325f, x, 1.0f));
-  const float e = __builtin_amdgcn_exp2f(u * u * -0.72134752044448170f);  // exp(-u^2 / 2)
-  float y = fmaf(-0.15001650154590607f, t, 0.5482092499732971f);
-  y = fmaf(y, t, -0.4863797724246979f);
-  y = fmaf(y, t, 0.5206797122955322f);
-  y = fmaf(y, t, -0.007771324831992388f);
-  y = fmaf(y, t, 0.21368199586868286f);
-  y = fmaf(y, t, 0.17792251706123352f);
-  y = fmaf(y, t, 0.18367408215999603f);
-  y = 0.5f * (y * t) * e;  // erfc(x) / 2
-  density = e * 0.39894228040143268f;
-  return u >= 0.0f ? 1.0f - y : y;
+// arithmetic, not HBM, bounded these kernels: 10 x 961 x 390 forward 17 us.)
+__device__ __forceinline__ float norm_tail(float u, float& e) {
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.2298097014427185f, fabsf(u), 1.0f));
+  e = __builtin_amdgcn_exp2f(u * u * -0.72134752044448170f);
+  float y = fmaf(-0.07500825077295303f, t, 0.27410462498664856f);
+  y = fmaf(y, t, -0.24318988621234894f);
+  y = fmaf(y, t, 0.2603398561477661f);
+  y = fmaf(y, t, -0.003885662415996194f);
+  y = fmaf(y, t, 0.10684099793434143f);
+  y = fmaf(y, t, 0.08896125853061676f);
+  y = fmaf(y, t, 0.09183704107999802f);
+  return (y * t) * e;
 }
 
 template <int ACT>
@@ -120,9 +117,9 @@ __device__ __forceinline__ float norm_act(float u) {
     sigmoid_pair(u, q, rest);
     return u * q;
   }
-  if (ACT == SLHIP_ACT_GELU) {
-    float density;
-    return u * norm_normal(u, density);
+  if (ACT == SLHIP_ACT_GELU) {  // u (1 - tail) or u tail: max(u, 0) - |u| tail; the tail is zero long before 64
+    float e;
+    return fmaf(-fminf(fabsf(u), 64.0f), norm_tail(u, e), fmaxf(u, 0.0f));
   }
   return u;
 }
@@ -135,21 +132,21 @@ __device__ __forceinline__ float norm_act_grad(float u) {
     return q * (1.0f + u * rest);
   }
   if (ACT == SLHIP_ACT_GELU) {
-    float density;
-    const float phi = norm_normal(u, density);
-    return fmaf(u, density, phi);
+    float e;
+    const float y = norm_tail(u, e);
+    return fmaf(u * 0.39894228040143268f, e, u >= 0.0f ? 1.0f - y : y);
   }
   return 1.0f;
 }
 // One element of either direction.
 template <int ACT>
 __device__ __forceinline__ float norm_out(float x, float mean, float rstd, float w, float b) {
-  return norm_act<ACT>(((x - mean) * rstd) * w + b);
+  return norm_act<ACT>(fmaf((x - mean) * rstd, w, b));
 }
 template <int ACT>
 __device__ __forceinline__ float norm_upstream(float x, float g, float mean, float rstd, float w, float b, float& hat) {
   hat = (x - mean) * rstd;
-  return g * norm_act_grad<ACT>(hat * w + b);
+  return g * norm_act_grad<ACT>(fmaf(hat, w, b));
 }
 
 // Where a workgroup works.  Its number walks the windows fastest, and numbers are dealt out so that an XCD gets a contiguous

@@ -209,6 +209,25 @@ def test_constant_groups_and_nan(hip, shape):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", [SILU, GELU])
+def test_activations_far_out(hip, kind):
+    """Weights from 10^-4 to 10^20: where the function is its argument, and where it is next to nothing."""
+    shape = (6, 1, 125, 1)
+    x, _, b, dy = data(shape, kind, tag=48)
+    w = (10.0 ** np.linspace(-4, 20, 125)).astype(np.float32)
+    out, mean, rstd = hip.group_norm(*shape, x, w, b, act=kind)
+    (want, _, _), (tol, _, _) = forward(shape, x, w, b, kind, 1e-5)
+    close(out, want, tol, "forward")
+    outs = [np.zeros(x.size, np.float32), np.zeros(125, np.float32), np.zeros(125, np.float32)]
+    hip.group_norm_grad(*shape, x, w, b, mean, rstd, dy, *outs, act=kind)
+    assert all(np.isfinite(o).all() for o in outs)
+    b[3], b[4] = np.inf, np.nan                            # in a bias they stay in their channel
+    got = hip.group_norm(*shape, x, w, b, act=kind)[0].reshape(6, 125)
+    assert (got[:, 3] == np.inf).all() and np.isnan(got[:, 4]).all()
+    assert np.array_equal(np.delete(got, (3, 4), axis=1), np.delete(out.reshape(6, 125), (3, 4), axis=1))
+
+
+@pytest.mark.gpu
 def test_gradients_against_differences(hip):
     shape = (2, 3, 6, 2)
     for kind in (NONE, SILU, GELU):
