@@ -38,6 +38,7 @@ struct NormArgs {
   unsigned chunks;        // runs of positions of a sample, a workgroup each
   size_t chunk;           // positions of a run
   size_t blocks;          // workgroups with work
+  bool by_xcd;            // windows share lines with their neighbours
   const float* x;
   const float* w;
   const float* b;
@@ -165,8 +166,12 @@ template <int V, int NT>
 __device__ __forceinline__ NormPlace norm_place(const NormArgs& a, bool backwards) {
   NormPlace p;
   const unsigned blocks = (unsigned)a.blocks, per = (blocks + 7) / 8;
-  unsigned id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  p.some = (blockIdx.x >> 3) < per && id < blocks;
+  unsigned id = blockIdx.x;
+  p.some = id < blocks;
+  if (a.by_xcd) {
+    id = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+    p.some = (blockIdx.x >> 3) < per && id < blocks;
+  }
   if (!p.some) id = 0;
   if (backwards) id = blocks - 1 - id;
   const unsigned cgv = (unsigned)(a.cg / V);
@@ -271,11 +276,12 @@ __device__ __forceinline__ NormTeam norm_team(const NormArgs& a, const NormPlace
 
 // Joins what the threads of a group know of it: `count` values of mean `here` whose squared differences from that add up to
 // `spread`.  Means are taken relative to the one of the group's first thread: it is the mean of many values itself, so
-// that no single value, however far from the others, stands between the sums and their difference.
+// that no single value, however far from the others, stands between the sums and their difference.  (Relative to zero where
+// that mean is within two of the thread's standard deviations of it: a small mean keeps its own digits then.)
 template <int V, int NT>
 __device__ __forceinline__ void norm_join(const NormArgs& a, const NormPlace& p, unsigned rank, float count, float here, float spread, float total,
                                           NormSums<NT>& s, float& mean, float& m2) {
-  if (p.active && rank == 0) s.reference[p.local] = here;
+  if (p.active && rank == 0) s.reference[p.local] = here * here * count > 4.0f * spread ? here : 0.0f;
   __syncthreads();
   const float reference = s.reference[p.local], away = here - reference;
   const float2 t = norm_group_sums<V, NT>(a, p, count * away, spread + count * (away * away), s);
@@ -880,6 +886,12 @@ __global__ __launch_bounds__(1024) void norm_columns_kernel(size_t rows, size_t 
 // ---------------------------------------------------------------- host side
 // Windows of about NORM_WINDOW vectors: whole groups, or pieces of one.
 constexpr size_t NORM_WINDOW = 32;
+// Whether windows begin or end within a 128-byte line, of which their neighbours have the rest.
+static bool norm_lines_shared(const NormArgs& a, int V) {
+  if (a.across == 1) return false;
+  const uintptr_t bases = (uintptr_t)a.x | (uintptr_t)a.out | (uintptr_t)a.g | (uintptr_t)a.dx;
+  return bases % 128 != 0 || a.C % 32 != 0 || a.lanes * (unsigned)V % 32 != 0 || (a.windows > 1 && a.cg % 32 != 0);
+}
 static void norm_windows(NormArgs& a, int V, unsigned threads) {
   const size_t cgv = a.cg / V;
   a.together = 1;
@@ -895,6 +907,7 @@ static void norm_windows(NormArgs& a, int V, unsigned threads) {
   a.across = (unsigned)((a.G + a.together - 1) / a.together * a.windows);
   a.rows = threads / a.lanes;
   if (a.rows > a.P) a.rows = (unsigned)a.P;
+  a.by_xcd = norm_lines_shared(a, V);
 }
 
 // Two pass: runs of positions such that the chip gets about 4096 workgroups and a thread still 8 positions.
@@ -930,6 +943,7 @@ static bool norm_fits(const slhip_ctx* ctx, NormArgs& a, int V, unsigned threads
   // Pieces of rows below 96 bytes cost more than the second reading does, unless all of it stays in the caches (forward at 64 x
   // 2048 x 320 in 32 groups, 40 bytes: 230 us here, 129 in two passes; 10 x 961 x 390 in 13, 120 bytes: 12 and 16; 32 x 1000 x
   // 64 in 8, 32 bytes but 8 MiB in all: 8 and 14).
+  a.by_xcd = norm_lines_shared(a, V);
   if (a.across > 1 && a.lanes * (size_t)V < 24 && a.N * a.P * a.C > (size_t(1) << 22)) return false;
   a.blocks = a.N * a.across;
   return true;

@@ -97,9 +97,12 @@ class HIP:
 
     def __init__(self, ordinal=0, cached=False):
         self.h = C.c_void_p()
+        self._optimisers = []
         _ck(lib().slh_device_new(ordinal, int(cached), C.byref(self.h)))
 
     def close(self):
+        for o in list(self._optimisers):
+            o.close()
         if self.h:
             lib().slh_device_free(self.h)
             self.h = None
@@ -315,19 +318,23 @@ class HIP:
 
 
 class AdamW:
-    """Handle of a device's AdamW optimiser; close it before the device."""
+    """Handle of a device's AdamW optimiser; it is closed with the device at the latest."""
 
     def __init__(self, dev, params, lr, beta1, beta2, eps, weight_decay, eight, seed):
-        self.h = C.c_void_p()
+        self.h, self.dev = C.c_void_p(), dev
         ids = (_u64 * len(params))(*[p.id for p in params])
         _ck(lib().slh_adamw_new(dev.h, _sz(len(params)), ids, _f(lr), _f(beta1), _f(beta2), _f(eps), _f(weight_decay), int(bool(eight)),
                                 _u64(seed), C.byref(self.h)))
+        dev._optimisers.append(self)
 
     def step(self):
+        if not self.h:
+            raise HostError("this optimiser is closed")
         _ck(lib().slh_adamw_step(self.h))
 
     def close(self):
         if self.h:
+            self.dev._optimisers.remove(self)
             _ck(lib().slh_adamw_free(self.h))
             self.h = None
 

@@ -255,12 +255,14 @@ def test_outputs_over_inputs_equal_separate_ones(hip, batch, steps, channels, mo
 @pytest.mark.gpu
 @pytest.mark.parametrize("mode", [LINEAR, SIGMOID])
 def test_two_contexts_on_two_streams(hip, mode):
-    """A context of its own and one on a stream of torch's, both busy with split sequences at once: each has its own workspace."""
-    import torch
+    """A context on a stream of its own and one on the caller's, both busy with split sequences at once: each has its own
+    workspace."""
     from sliced_amd.device import Context
     batch, steps, channels = 1, 9000, 40
-    stream = torch.cuda.Stream()
-    one, two = Context(0), Context(0, stream=stream.cuda_stream)
+    runtime = C.CDLL("libamdhip64.so.7")               # (the one the library has loaded)
+    stream = C.c_void_p()
+    assert runtime.hipStreamCreateWithFlags(C.byref(stream), 1) == 0
+    one, two = Context(0), Context(0, stream=stream.value)
     sets = [data(mode, batch, steps, channels, tag=60 + 5 * k) for k in range(2)]
     want = [hip.gated_scan(mode, batch, steps, channels, *s)[0] for s in sets]
     bufs = [[c.array(a) for a in s] + [c.empty(s[0].size)] for c, s in zip((one, two), sets)]
@@ -273,6 +275,8 @@ def test_two_contexts_on_two_streams(hip, mode):
     for c, b in zip((one, two), bufs):
         for k in b:
             k.free()
+        c.close()
+    assert runtime.hipStreamDestroy(stream) == 0
 
 
 @pytest.mark.gpu

@@ -225,6 +225,9 @@ def test_adamw_errors_on_the_tape():
         with pytest.raises(host.HostError):           # no gradient yet
             opt.step()
         opt.close()
+        with pytest.raises(host.HostError):
+            opt.step()
+        left = d.adamw([b])                           # closed with the device
         d.add(a, b).backward()
         twice = d.adamw([a, a])
         with pytest.raises(host.HostError, match="overlap"):
@@ -237,3 +240,6 @@ def test_adamw_errors_on_the_tape():
         with pytest.raises(host.HostError):
             host.mlp_train(0, 8, 1, 4, 1, np.zeros(8, np.float32), np.zeros(8, np.float32), host.mlp_init(0, 1, 4, 1), 1e-3, 1, whole_step=True,
                            optimizer="adamw")
+    left.close()
+    with pytest.raises(host.HostError):
+        left.step()
