@@ -15,6 +15,9 @@
 //            of their own, and the second kernel starts where the first one ended, with what the last-level cache still
 //            holds.
 //
+// Measured: 8192 rows x 2048 in 16 groups backward 44 us (4.6 TB/s), 32 x 1024 x 512 in 32 groups forward on chip 26 us (5.2
+// TB/s), 32 x 4096 x 512 in two passes forward 131 us (6.2 TB/s of the 12 bytes that those move), backward 240 (5.6 of 20).
+//
 // In the latter two a window is a run of whole groups, about 32 vectors of channels wide (512 bytes of a row of x): narrower
 // pieces of rows than that cost HBM bandwidth.  Groups wider than a workgroup are cut.  A thread keeps to one vector of V
 // channels and steps through the positions, so that weights, biases and per-channel sums stay in registers.  V is the

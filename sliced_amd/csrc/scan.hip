@@ -8,7 +8,9 @@
 // G_t = a_t d_t, so that a step needs its own gate only: d_t = dh_t + G_{t+1}, G_t = a_t d_t - the same recurrence
 // run from the last step to the first, with input a_t dh_t.
 //
-// HBM is the bound: 12 bytes an element forward, 20 (linear) or 24 (sigmoid) backward.
+// HBM is the bound: 12 bytes an element forward, 20 (linear) or 24 (sigmoid) backward.  Measured: 32 x 1000 x 1024 forward
+// 73 us (5.4 TB/s), backward 152 (5.2); 8 x 2048 x 1024 forward 47 us (4.2), backward 88 (4.6); 65536 x 1024 linear 231 us
+// (5.8 TB/s of the 20 bytes that its split moves); 32 x 1 x 2048, a token, 2.8 us in the kernel.
 #include <type_traits>
 
 #include "common.hpp"
@@ -35,7 +37,7 @@ struct ScanArgs {
 
 // V neighbouring channels of a lane.  Where the last lanes of a row would reach past its end they move back to its last V
 // channels and store only those that no other lane owns (from `skip` on): every load is a whole vector without a branch
-// around it - with one the loads of a run waited for each other (4 x 4099 x 1008 backward: 145 us, 105 without).
+// around it - with one the loads of a run waited for each other (4 x 4099 x 1001 backward: 193 us, 100 without).
 template <int V>
 struct ScanVec {
   float v[V];
@@ -362,7 +364,8 @@ __device__ __forceinline__ void scan_identity(ScanVec<V>& A, ScanVec<V>& H) {
   }
 }
 
-// The pair of every chunk but the last: A run of consecutive steps to each group of L threads.
+// The pair of every chunk but the last: a run of consecutive steps to each group of L threads.  (5.9 TB/s at 65536 x 1024; 8
+// or 16 rows requested at a time instead of 4 change nothing.)
 template <bool GRAD, int MODE, int V, int L, int R, int NT>
 __global__ __launch_bounds__(NT) void scan_totals_kernel(ScanArgs a, ScanSplit s) {
   constexpr int NW = NT / 64, RUNS = NT / L;
@@ -511,11 +514,12 @@ static int32_t scan_launch_tiles(slhip_ctx* ctx, const ScanArgs& a) {
     set_error("slhip_gated_scan: too many channels for one launch");
     return SLHIP_EINVAL;
   }
-  ScanSplit s = {a.steps, nullptr, nullptr, a.channels % 32 != 0 || ((uintptr_t)a.gate | (uintptr_t)a.x | (uintptr_t)(GRAD ? a.dx : a.h_out)) % 128 != 0};
+  const uintptr_t bases = (uintptr_t)a.gate | (uintptr_t)a.x | (uintptr_t)(GRAD ? a.dx : a.h_out);
+  ScanSplit s = {a.steps, nullptr, nullptr, a.channels % 32 != 0 || bases % 128 != 0};
   size_t chunks = 1;
   const size_t state = a.batch * a.channels;
   if (groups < (size_t)ctx->num_cu) {
-    // two workgroups to a CU, each with a tile at least (65536 x 1024 forward, 8 groups: 64 chunks 220 us, 32 227, 128 225)
+    // two workgroups to a CU, each with a tile at least (65536 x 1024 forward, 8 groups: 64 chunks 232 us, 32 238)
     chunks = ((size_t)ctx->num_cu * 2 + groups - 1) / groups;
     const size_t most = a.steps / TILE;
     if (chunks > most) chunks = most;
@@ -542,13 +546,15 @@ static int32_t scan_launch_tiles(slhip_ctx* ctx, const ScanArgs& a) {
 template <bool GRAD, int MODE>
 static int32_t scan_launch(slhip_ctx* ctx, const ScanArgs& a) {
   // steps of a run, and threads: forward longer runs and more of them, backward holds twice the arrays in registers
-  // (8 x 2048 x 1024: forward 4 and 512 46 us, 4 and 256 58, 2 and 512 58; backward 2 and 256 85 us, 2 and 512 91, 4 and 256 90)
+  // (8 x 2048 x 1024: forward 4 and 512 41.4 us, 4 and 256 43.2, 2 and 512 41.5, which loses where steps are split; backward 2
+  // and 256 89.8 us, 2 and 512 91.9, 4 and 256 93.1)
   constexpr int R = GRAD ? 2 : 4, NT = GRAD ? 256 : 512;
   if (a.steps > 8) {
     if (a.channels > 32) {
-      // Wide channel tiles, 512 bytes of a row, are what HBM likes best (32 x 1000 x 1024 backward: 151 us at 512 bytes, 168 at
-      // 256, 187 at 128), if there are enough of them; narrow ones fill the chip where a split of the steps, which reads the
-      // inputs of the recurrence twice, would have to otherwise (8 x 2048 x 1024: forward 46 us narrow, 69 wide and split).
+      // Wide channel tiles, 512 bytes of a row, are what HBM likes best (32 x 1000 x 1024 backward: 151 us at 512 bytes, 167 at
+      // 256, 180 at 128; forward 74, 81, 92), if there are enough of them; narrow ones fill the chip where a split of the steps, which reads the
+      // inputs of the recurrence twice, would have to otherwise (forward 8 x 2048 x 1024 narrow 47 us, 4 x 4099 x 1024, which has
+      // as many elements and too few narrow tiles, wide and split 67).
       const size_t cu = (size_t)ctx->num_cu, wide = a.batch * ((a.channels + 127) / 128), narrow = a.batch * ((a.channels + 31) / 32);
       if (a.channels > 64 && (wide >= cu || narrow < cu || a.steps < 256)) return scan_launch_tiles<GRAD, MODE, 4, 32, R, NT>(ctx, a);
       return scan_launch_tiles<GRAD, MODE, 4, 8, R, NT>(ctx, a);
