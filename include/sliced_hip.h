@@ -277,7 +277,8 @@ int32_t slhip_group_norm_grad(slhip_ctx* ctx, size_t samples, size_t positions, 
  * or gate itself and, with steps = 1, h0 itself; any other overlap is refused (SLHIP_EALIAS).
  * Long sequences are cut into runs that are joined by their products of gates, in a fixed order.  For
  * SLHIP_SCAN_LINEAR a product of gates over a run of steps has to be representable: gates of magnitude
- * up to one always are.
+ * up to one always are.  Rows that hold several sequences: gate 0 (LINEAR) or −inf (SIGMOID) forgets a finite
+ * state before it exactly; padding: gate 1 with x 0, or +inf with any finite x, keeps the state.
  * slhip_gated_scan_grad: with h_grad (and h_last_grad, which may be NULL) given and h as the forward call left it,
  * d_t = h_grad_t + a_{t+1}·d_{t+1} (a = gate or s; d_{steps-1} also takes h_last_grad):
  *     LINEAR   gate_grad = d·h_{t−1}                   x_grad = d
