@@ -179,12 +179,14 @@ __device__ __forceinline__ unsigned adamw_exponent(float x) {
   return e == 0xffu ? 0u : e;
 }
 
-// v's value in units of its scale, stochastically rounded to two bits behind the leading one: r16 / 2^16 of the spacing
-// is added before the rest is cut off.  What is left is what E5M2 holds, down to its smallest normal value; below that
-// the conversion rounds the remaining bits to nearest.
+// v's value in units of its scale, stochastically rounded to E5M2: r16 / 2^16 of the format's spacing is added before the
+// rest is cut off.  That spacing is a quarter of the leading bit down to the smallest normal value, 2^-14, and 2^-16 below it;
+// with 2^-14 added a value from below lies in the binade whose quarter is 2^-16, so that one cut does for both.  What is left
+// is what the format holds: the conversion rounds nothing.  (Two bits behind the leading one everywhere, the rest left to the
+// conversion, would round twice below 2^-14, the second time to nearest: 2 and 4 units of 2^-16 then never decay.)
 __device__ __forceinline__ float adamw_round_v(float y, unsigned r16) {
-  const unsigned b = __float_as_uint(y);
-  const float cut = __uint_as_float((b + (r16 << 5)) & ~0x1fffffu);
+  const float o = y < 6.103515625e-05f ? 6.103515625e-05f : 0.0f;  // 2^-14
+  const float cut = __uint_as_float((__float_as_uint(y + o) + (r16 << 5)) & ~0x1fffffu) - o;
   return y > 0.0f && y < __builtin_huge_valf() ? fmaxf(cut, 1.52587890625e-05f) : y;  // 2^-16, E5M2's smallest
 }
 
