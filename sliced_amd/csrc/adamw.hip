@@ -183,11 +183,12 @@ __device__ __forceinline__ unsigned adamw_exponent(float x) {
 // rest is cut off.  That spacing is a quarter of the leading bit down to the smallest normal value, 2^-14, and 2^-16 below it;
 // with 2^-14 added a value from below lies in the binade whose quarter is 2^-16, so that one cut does for both.  What is left
 // is what the format holds: the conversion rounds nothing.  (Two bits behind the leading one everywhere, the rest left to the
-// conversion, would round twice below 2^-14, the second time to nearest: 2 and 4 units of 2^-16 then never decay.)
-__device__ __forceinline__ float adamw_round_v(float y, unsigned r16) {
+// conversion, would round twice below 2^-14, the second time to nearest: 2 and 4 units of 2^-16 then never decay.)  y = v / scale is zero
+// where v is some 2^164 below the block's largest: whether there is a v is asked of v itself.
+__device__ __forceinline__ float adamw_round_v(float v, float y, unsigned r16) {
   const float o = y < 6.103515625e-05f ? 6.103515625e-05f : 0.0f;  // 2^-14
   const float cut = __uint_as_float((__float_as_uint(y + o) + (r16 << 5)) & ~0x1fffffu) - o;
-  return y > 0.0f && y < __builtin_huge_valf() ? fmaxf(cut, 1.52587890625e-05f) : y;  // 2^-16, E5M2's smallest
+  return v > 0.0f && y < __builtin_huge_valf() ? fmaxf(cut, 1.52587890625e-05f) : y;  // 2^-16, E5M2's smallest
 }
 
 __global__ __launch_bounds__(256) void adamw8_kernel(Adamw8Args a) {
@@ -263,7 +264,7 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Adamw8Args a) {
     const uint64_t word = adamw_mix(key + i / 4);
     float y[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) y[k] = adamw_round_v(v[k] * iv, (unsigned)(word >> (16 * k)) & 0xffffu);
+    for (int k = 0; k < 4; ++k) y[k] = adamw_round_v(v[k], v[k] * iv, (unsigned)(word >> (16 * k)) & 0xffffu);
     int mc = __builtin_amdgcn_cvt_pk_fp8_f32(m[0] * im, m[1] * im, 0, false);
     mc = __builtin_amdgcn_cvt_pk_fp8_f32(m[2] * im, m[3] * im, mc, true);
     int vc = __builtin_amdgcn_cvt_pk_bf8_f32(y[0], y[1], 0, false);

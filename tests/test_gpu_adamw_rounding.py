@@ -23,7 +23,7 @@ def encode(m, v, r16):
     x, y = m / np.repeat(sm, 256)[:m.size], v / np.repeat(sv, 256)[:m.size]
     low = np.where(y < NORMAL, NORMAL, np.float32(0))
     cut = (((y + low).view(np.uint32) + (r16 << 5)) & ~np.uint32(0x1FFFFF)).view(np.float32) - low
-    y = np.where(y > 0, np.maximum(cut, SMALLEST), y).astype(np.float32)
+    y = np.where(v > 0, np.maximum(cut, SMALLEST), y).astype(np.float32)
     code = lambda a, kind: torch.from_numpy(a).to(kind)  # noqa: E731
     v8 = code(y, torch.float8_e5m2)
     assert np.array_equal(v8.float().numpy(), y, equal_nan=True)          # the conversion rounds nothing
@@ -107,3 +107,21 @@ def test_v_decays_whatever_its_part_of_the_block(hip):
         allowed, want = 5 * np.sqrt(0.3 * s * d / v.shape[1]) + 300 * 2.0 ** -16 * d, s * base.f32(0.999) ** 300
         base.say("v of", s, "units:", v[k].mean(), "expected", want)
         assert -allowed <= v[k].mean() - want <= allowed + (0.26 if s < 4 else 0), s
+
+
+@pytest.mark.gpu
+def test_a_v_that_underflows_beside_the_largest_is_not_zero(hip):
+    """Gradients whose squares are 2^330 apart in one block: the small ones' v is zero in units of the scale, and is kept as the
+    smallest value all the same."""
+    n = 600
+    g = np.full(n, 1e-19, np.float32)
+    g[[0, 300]] = 3e10
+    g[10:20] = 0
+    p, (m8, v8, scales) = [np.zeros(n, np.float32)], base.zeros8([n])
+    hip.adamw8_step_multi(p, [g], m8, v8, scales, step=1, seed=SEED, **HYPER)
+    r1, r2 = np.float32(1) - np.float32(0.9), np.float32(1) - np.float32(0.999)
+    v = (g * r2) * g
+    assert ((v > 0) == (g > 0)).all() and v[1] / scales[0][1] == 0
+    for got, w, what in zip((m8[0], v8[0], scales[0]), encode(g * r1, v, base.random16(n, 0, 1, SEED)), ("m8", "v8", "scales")):
+        assert np.array_equal(got, w), what
+    assert ((v8[0] > 0) == (g > 0)).all()
