@@ -334,7 +334,8 @@ __global__ __launch_bounds__(256) void norm_stats_kernel(NormArgs a) {
       }
     const float all = count + U * V, away = m - here, part = (U * V) * __builtin_amdgcn_rcpf(all);
     here = fmaf(away, part, here);
-    spread += fmaf(away * away, count * part, q);
+    // (the first values of a thread join nothing: the square of their mean may be infinite, and 0 of it no number)
+    spread += count > 0.0f ? fmaf(away * away, count * part, q) : q;
     count = all;
   });
   const unsigned rank = norm_team<V>(a, p).rank;
