@@ -251,7 +251,8 @@ int32_t slhip_softmax_grad(slhip_ctx* ctx, size_t samples, size_t features, floa
  * groups = 1 and positions = 1 is a layer norm of every row.  weight and bias (channels each) may be
  * NULL (ones, zeros).  mean and rstd (samples × groups each) receive what the backward pass needs and
  * may be NULL.  out may be x itself; any other overlap with an input is refused (SLHIP_EALIAS).  At most 2^31 − 1
- * channels.
+ * channels.  A group whose magnitudes add up to a float but whose squared deviations do not (some 10^19 away from the mean)
+ * has an infinite variance: rstd 0, out = act(bias).
  * slhip_group_norm_grad, with g = out_grad ⊙ act'(u), hat = (x − mean)·rstd, gx = g·weight, < > a mean over the
  * sample's group:
  *     x_grad      = beta·x_grad + rstd·(gx − <gx> − hat·<gx·hat>)

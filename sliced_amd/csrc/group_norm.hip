@@ -263,6 +263,14 @@ __device__ __forceinline__ float2 norm_group_sums(const NormArgs& a, const NormP
   return s.total[p.local];
 }
 
+// Squared differences from another mean: q of them from one, whose distances from it add up to `sum`, less what a move by `shift` to
+// the mean takes off; rounding may not make them negative.  Where the squares pass the largest float they stay infinite in every
+// kernel - 1/sqrt(var) is zero then - although the difference is one of infinities; NaN stays NaN.
+__device__ __forceinline__ float norm_moved(float q, float sum, float shift) {
+  const float rest = q - sum * shift;
+  return rest > 0.0f ? rest : q < __builtin_huge_valf() ? 0.0f : q;
+}
+
 // A working thread's place among those of its group in the workgroup.
 struct NormTeam {
   unsigned rank, size;
@@ -290,8 +298,7 @@ __device__ __forceinline__ void norm_join(const NormArgs& a, const NormPlace& p,
   const float2 t = norm_group_sums<V, NT>(a, p, count * away, spread + count * (away * away), s);
   const float shift = t.x / total;
   mean = reference + shift;
-  m2 = fmaxf(t.y - t.x * shift, 0.0f);
-  if (t.y != t.y) m2 = t.y;  // (fmaxf would lose a NaN)
+  m2 = norm_moved(t.y, t.x, shift);
 }
 
 // A thread's positions, several of them requested at a time: 64 bytes of each array, or 32 of narrow vectors.
@@ -366,10 +373,8 @@ __global__ __launch_bounds__(256) void norm_apply_kernel(NormArgs a) {
     s2 += fmaf(count, away * away, in[2 * i + 1]);
   }
   const float2 both = norm_group_sums<V, 256>(a, p, s1, s2, sums);
-  const float mean = reference + both.x / total;
-  float var = (both.y - both.x * (both.x / total)) / total;
-  if (var < 0.0f) var = 0.0f;
-  const float rstd = 1.0f / sqrtf(var + a.eps);
+  const float shift = both.x / total, mean = reference + shift;
+  const float rstd = 1.0f / sqrtf(norm_moved(both.y, both.x, shift) / total + a.eps);
   if (!p.active) return;
   if (p.part == 0 && t.rank == 0) {
     if (a.mean) a.mean[p.n * a.G + p.g] = mean;

@@ -27,3 +27,29 @@ def test_a_mean_whose_square_overflows(hip, shape):
     out, mean, rstd = hip.group_norm(*shape, same, w, b, act=NONE)
     assert np.array_equal(out.reshape(x.shape), np.broadcast_to(b, x.shape)) and (mean == same.flat[0]).all()
     assert np.allclose(rstd, 1e-5 ** -0.5, rtol=4 * U)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES)
+def test_deviations_whose_squares_overflow(hip, shape):
+    """Deviations near 10^20: the variance is infinite, 1/sqrt(var) zero, the outputs what the biases give, and the gradients zero
+    but for the biases'.  A group beside it, of ordinary values, does not notice."""
+    base.say("norm, infinite variance", shape)
+    n, p, c, g = shape
+    x, w, b, dy = base.data(shape, SILU, tag=210, offset=0.0)
+    plain = x.copy()
+    x[0, :, :c // g] *= np.float32(1e20)                     # the first group of the first sample
+    for act in (NONE, SILU):
+        out, mean, rstd = hip.group_norm(*shape, x, w, b, act=act)
+        (want, wm, wr), (tol, tm, tr) = base.forward(shape, plain, w, b, act, 1e-5)
+        big = x[0, :, :c // g].astype(np.float64)
+        want[0, :, 0], tol[0, :, 0] = base.act(act, b[:c // g].astype(np.float64)), 6 * U * np.abs(b[:c // g])
+        wm[0, 0], tm[0, 0] = big.mean(), base.CHAIN * U * np.abs(big).mean()
+        wr[0, 0], tr[0, 0] = 0, 0
+        for got, v, t, what in zip((out, mean, rstd), (want, wm, wr), (tol, tm, tr), ("out", "mean", "rstd")):
+            base.close(got, v, t, what)
+        grads = [np.full(x.size, np.nan, np.float32), np.full(c, np.nan, np.float32), np.full(c, np.nan, np.float32)]
+        hip.group_norm_grad(*shape, x, w, b, mean, rstd, dy, *grads, act=act)
+        for got, v, t, what in zip(grads, *base.backward(shape, x, w, b, act, mean, rstd, dy), ("x", "weight", "bias")):
+            base.close(got, v, t, what)
+        assert (grads[0].reshape(x.shape)[0, :, :c // g] == 0).all()
