@@ -393,8 +393,8 @@ int32_t slhip_sgd_step_multi(slhip_ctx* ctx, size_t count, float* const* params,
  * as zeros.  t is `step`, counted from 1; or, with step = 0, the counter that step_dev (a device
  * pointer, 8-byte aligned, starting at zero) names, which the call advances by one first: that is the
  * form for recorded steps, whose replays must not repeat one t (one more small launch, which leaves
- * what it computes in the workspace).  No array that the call writes may overlap any other
- * (SLHIP_EALIAS); count is at most 16384.  beta1 and beta2 lie in [0, 1), eps >= 0.
+ * what it computes in the workspace).  No array that the call writes, the counter among them, may
+ * overlap any other (SLHIP_EALIAS); count is at most 16384.  beta1 and beta2 lie in [0, 1), eps >= 0.
  * slhip_adamw8_step_multi keeps the moments in 8 bits: m8[i] holds lens[i] OCP E4M3 values, v8[i] lens[i]
  * OCP E5M2 values (both 4-byte aligned), and scales[i] two floats, m's and v's, for every started block
  * of 256 elements; a moment is its 8-bit value times its block's scale, a power of two.  All start as

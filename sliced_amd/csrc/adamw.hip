@@ -289,37 +289,40 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Adamw8Args a) {
   }
 }
 
-// The arrays of a call, in the order of their addresses: 2^47 of those and 2^17 arrays make one 64-bit key, whose sorting
-// takes 2 us for 64 tensors.
+// The arrays of a call, in the order of their addresses: 2^47 of those and 2^17 arrays make one 64-bit key.
 constexpr size_t ADAMW_MOST = 16384;  // tensors of a call
-static_assert(5 * ADAMW_MOST <= (size_t(1) << 17), "arrays of a call");
+static_assert(5 * ADAMW_MOST + 1 <= (size_t(1) << 17), "arrays of a call");
 
 // Whether an array that the call writes shares memory with any other.  `arrays` kinds of `count` pointers each; bytes(kind, i)
-// is an array's length, `read_only` the kind that is not written.
+// is an array's length, `read_only` the kind that is not written.  The counter of steps, if there is one, comes behind them.
 template <class F>
-static int32_t adamw_overlap(const char* who, const void* const* const* arrays, int kinds, int read_only, size_t count, F&& bytes) {
-  uint64_t few[5 * ADAMW_TENSORS];
+static int32_t adamw_overlap(const char* who, const void* const* const* arrays, int kinds, int read_only, size_t count, const uint64_t* counter,
+                             F&& bytes) {
+  uint64_t few[5 * ADAMW_TENSORS + 1];
   uint64_t* keys = few;
-  const size_t n = count * (size_t)kinds;
+  const size_t all = count * (size_t)kinds, n = all + (counter ? 1 : 0);
   if (count > ADAMW_TENSORS && !(keys = new (std::nothrow) uint64_t[n])) {
     set_error("%s: out of host memory", who);
     return SLHIP_EINVAL;
   }
   size_t k = 0;
   uint64_t high = 0;
+  auto take = [&](const void* p) {
+    const uint64_t at = (uint64_t)(uintptr_t)p;
+    high |= at >> 47;
+    keys[k] = at << 17 | k;
+    ++k;
+  };
   for (int kind = 0; kind < kinds; ++kind)
-    for (size_t i = 0; i < count; ++i, ++k) {
-      const uint64_t at = (uint64_t)(uintptr_t)arrays[kind][i];
-      high |= at >> 47;
-      keys[k] = at << 17 | k;
-    }
+    for (size_t i = 0; i < count; ++i) take(arrays[kind][i]);
+  if (counter) take(counter);
   std::sort(keys, keys + n);
   uint64_t any = 0, written = 0;  // where the arrays so far end, and those of them that are written
   bool shared = false;
   for (size_t i = 0; i < n; ++i) {
     const uint64_t at = keys[i] >> 17, which = keys[i] & ((1u << 17) - 1);
     const int kind = (int)(which / count);
-    const uint64_t end = at + bytes(kind, (size_t)(which % count));
+    const uint64_t end = at + (which == all ? sizeof(uint64_t) : bytes(kind, (size_t)(which % count)));
     const bool writes = kind != read_only;
     shared = shared || at < (writes ? any : written);
     if (any < end) any = end;
@@ -395,7 +398,7 @@ SLHIP_API int32_t slhip_adamw_step_multi(slhip_ctx* ctx, size_t count, float* co
     SLHIP_REQUIRE(lens[i] <= ADAMW_LONGEST, "tensor too long");
   }
   const void* const* const arrays[] = {(const void* const*)params, (const void* const*)grads, (const void* const*)m, (const void* const*)v};
-  int32_t rc = adamw_overlap("slhip_adamw_step_multi", arrays, 4, 1, count, [&](int, size_t i) { return lens[i] * sizeof(float); });
+  int32_t rc = adamw_overlap("slhip_adamw_step_multi", arrays, 4, 1, count, step_dev, [&](int, size_t i) { return lens[i] * sizeof(float); });
   if (rc) return rc;
   SLHIP_ON_DEVICE(ctx);
   AdamwArgs a;
@@ -427,7 +430,7 @@ SLHIP_API int32_t slhip_adamw8_step_multi(slhip_ctx* ctx, size_t count, float* c
   }
   const void* const* const arrays[] = {(const void* const*)params, (const void* const*)grads, (const void* const*)m8, (const void* const*)v8,
                                        (const void* const*)scales};
-  int32_t rc = adamw_overlap("slhip_adamw8_step_multi", arrays, 5, 1, count, [&](int kind, size_t i) {
+  int32_t rc = adamw_overlap("slhip_adamw8_step_multi", arrays, 5, 1, count, step_dev, [&](int kind, size_t i) {
     return kind < 2 ? lens[i] * sizeof(float) : kind < 4 ? lens[i] : (lens[i] + ADAMW_BLOCK - 1) / ADAMW_BLOCK * 2 * sizeof(float);
   });
   if (rc) return rc;
