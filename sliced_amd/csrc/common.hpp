@@ -203,14 +203,15 @@ __device__ __forceinline__ void st1s(float* p, float v) { __builtin_nontemporal_
 // 1/(1 + exp(-z)) and 1/(1 + exp(z)), which add up to one, each to about two units in its last place at either end: with
 // e = exp(-|z|) nothing overflows, and the smaller of the two is e / (1 + e), not a difference.  The hardware's 2^x and
 // reciprocal with a correction each (the rounding of |z| log2(e) is put back as a factor 1 + lo ln 2; one Newton step):
-// half the instructions of the library's exponential and the IEEE quotient.
+// half the instructions of the library's exponential and the IEEE quotient.  The hardware's 2^x has no results below 2^-126
+// other than zero: those, from |z| = 87.3 on, are taken 2^64 larger and scaled back, down to the smallest float at 103.9.
 __device__ __forceinline__ void sigmoid_pair(float z, float& s, float& rest) {
-  float t = fabsf(z);
-  t = t > 150.0f ? 150.0f : t;  // keeps NaN; e is zero from 104 on
+  const float t = __builtin_elementwise_minimum(fabsf(z), 150.0f);  // NaN stays NaN; e is zero by then
   const float hi = -t * 1.44269502162933349609375f;                                   // log2(e), rounded
   const float lo = fmaf(-t, 1.925963033500011079e-8f, fmaf(-t, 1.44269502162933349609375f, -hi));  // and what that left
-  const float e0 = __builtin_amdgcn_exp2f(hi);
-  const float e = fmaf(e0, lo * 0.693147180559945309f, e0);
+  const bool tiny = hi < -126.0f;
+  const float e0 = __builtin_amdgcn_exp2f(hi + (tiny ? 64.0f : 0.0f));                // (the sum is exact)
+  const float e = fmaf(e0, lo * 0.693147180559945309f, e0) * (tiny ? 5.42101086242752217e-20f : 1.0f);  // 2^-64
   const float d = 1.0f + e, r0 = __builtin_amdgcn_rcpf(d);
   const float big = fmaf(fmaf(-d, r0, 1.0f), r0, r0), small = e * big;
   s = z >= 0.0f ? big : small;
