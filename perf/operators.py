@@ -133,7 +133,7 @@ def prepare(case, seed):
     def uniform(*shape):
         return torch.rand(*shape, generator=g, device=DEV)
 
-    s = {"case": dict(case)}
+    s = {"case": dict(case, stream=(torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream))}
     if case["op"] == "adamw":
         lens = _lens(case)
         starts, total = _starts(lens)
@@ -351,19 +351,20 @@ def _adamw_outputs(s):
 
 
 # ---------------------------------------------------------------- the library's calls
-_context = None
+_contexts = {}
 
 
-def _ctx():
-    global _context
-    if _context is None:
+def _ctx(stream):
+    """The library's context for a device's stream, the one that a state's inputs were made on: calls come behind them."""
+    if stream not in _contexts:
         from sliced_amd.device import Context
-        _context = Context(0, stream=torch.cuda.current_stream().cuda_stream)
-    return _context
+        _contexts[stream] = Context(stream[0], stream=stream[1])
+    return _contexts[stream]
 
 
 def _run_own(s):
-    c, ctx = s["case"], _ctx()
+    c = s["case"]
+    ctx = _ctx(c["stream"])
     if c["op"] == "adamw":
         if c["bits"] == 32:
             ctx.call("slhip_adamw_step_multi", s["count"], *s["args"], s["lens"], LR, BETA1, BETA2, EPS, DECAY, s["t"], None)
