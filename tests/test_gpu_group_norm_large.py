@@ -1,6 +1,6 @@
 """Group norm of values whose squares, or whose squared deviations, do not fit 32 bits: every route through the kernels gives the
 same answer.  The shapes go to the rows of a wave, of a workgroup of 256 and of 1024, to the on-chip kernels of 256 and of 1024
-threads, and to two passes with one part a group, several runs of positions, and groups cut into windows."""
+threads, and to two passes with several runs of positions, and with groups cut into windows."""
 import numpy as np
 import pytest
 
