@@ -251,8 +251,8 @@ int32_t slhip_softmax_grad(slhip_ctx* ctx, size_t samples, size_t features, floa
  * groups = 1 and positions = 1 is a layer norm of every row.  weight and bias (channels each) may be
  * NULL (ones, zeros).  mean and rstd (samples × groups each) receive what the backward pass needs and
  * may be NULL.  out may be x itself; any other overlap with an input is refused (SLHIP_EALIAS).  At most 2^31 − 1
- * channels.  A group whose magnitudes add up to a float but whose squared deviations do not (some 10^19 away from the mean)
- * has an infinite variance: rstd 0, out = act(bias).
+ * channels.  A group whose magnitudes add up to a float but whose squared deviations do not (values some
+ * 10^19 away from their mean) has an infinite variance: rstd 0, out = act(bias).
  * slhip_group_norm_grad, with g = out_grad ⊙ act'(u), hat = (x − mean)·rstd, gx = g·weight, < > a mean over the
  * sample's group:
  *     x_grad      = beta·x_grad + rstd·(gx − <gx> − hat·<gx·hat>)
@@ -278,8 +278,9 @@ int32_t slhip_group_norm_grad(slhip_ctx* ctx, size_t samples, size_t positions, 
  * or gate itself and, with steps = 1, h0 itself; any other overlap is refused (SLHIP_EALIAS).
  * Long sequences are cut into runs that are joined by their products of gates, in a fixed order.  For
  * SLHIP_SCAN_LINEAR a product of gates over a run of steps has to be representable: gates of magnitude
- * up to one always are.  Rows that hold several sequences: gate 0 (LINEAR) or −inf (SIGMOID) forgets a finite
- * state before it exactly; padding: gate 1 with x 0, or +inf with any finite x, keeps the state.
+ * up to one always are (where such a product is zero, an infinite state before the run becomes NaN in it).
+ * Rows that hold several sequences: gate 0 (LINEAR) or −inf (SIGMOID) forgets a finite state before it
+ * exactly; padding: gate 1 with x 0, or +inf with any finite x, keeps the state.
  * slhip_gated_scan_grad: with h_grad (and h_last_grad, which may be NULL) given and h as the forward call left it,
  * d_t = h_grad_t + a_{t+1}·d_{t+1} (a = gate or s; d_{steps-1} also takes h_last_grad):
  *     LINEAR   gate_grad = d·h_{t−1}                   x_grad = d
@@ -401,8 +402,10 @@ int32_t slhip_sgd_step_multi(slhip_ctx* ctx, size_t count, float* const* params,
  * zeros.  The update uses the moments before they are rounded.  m is rounded to nearest, v
  * stochastically (rounded to nearest, a decay of 0.1 % a step would never leave the spacing of 8 bits),
  * with random bits that depend on seed, t, the tensor's place in the list and the element alone; a v
- * that is not zero never rounds to zero.  Infinite and NaN moments stay in their own element (E4M3 has no
- * infinity: an infinite m is kept as NaN). */
+ * that is not zero never rounds to zero.  An m of less than about 2^-14 of its block's largest is at E4M3's last
+ * four values, where a decay of 10 % rounds back to what it was: an element that gets no gradient any more, in
+ * a block whose others do, goes on moving by about lr a step (its v decays to 2^-30 of the block's largest).  Infinite
+ * and NaN moments stay in their own element (E4M3 has no infinity: an infinite m is kept as NaN). */
 int32_t slhip_adamw_step_multi(slhip_ctx* ctx, size_t count, float* const* params, const float* const* grads,
                                float* const* m, float* const* v, const size_t* lens, float lr, float beta1, float beta2,
                                float eps, float weight_decay, uint64_t step, uint64_t* step_dev);

@@ -5,7 +5,7 @@
 //
 // Every element is read and written once and nothing is reduced but the blocks' largest magnitudes, so
 // HBM is the bound: 28 bytes an element with f32 moments (p, m, v in and out, g in), 16 with 8-bit ones.  Measured: 40 M
-// elements in 150 tensors 190 us (5.9 TB/s, three launches), 134 M with 8-bit moments 345 us (6.2 TB/s), 5.8 M 19 us (4.9),
+// elements in 150 tensors 190 us (5.9 TB/s, three launches), 134 M with 8-bit moments 345 us (6.2 TB/s), 5.8 M 19.5 us (4.8),
 // the six tensors of a net of 4353 parameters 3.1 us in the kernel.
 //
 // A launch takes up to 64 tensors: their pointers and the number of each one's first workgroup travel in
@@ -17,7 +17,8 @@
 // power of two: scaling is then exact both ways and the only rounding is to the 8-bit format.  (A float
 // format wants the scale for its range, not for its precision: a power of two loses nothing.)  m is rounded
 // to nearest.  v is rounded stochastically: at b2 = 0.999 its decay of 0.1 % a step is far below half the
-// spacing of any 8-bit format, so rounded to nearest it would never decay.  The random bits come from the
+// spacing of any 8-bit format, so rounded to nearest it would never decay.  (m's decay of 10 % is more than half the spacing
+// down to four units of the smallest, 2^-14 of the block's largest m; what is below that stays, while that one does.)  The random bits come from the
 // counter-based generator of slhip_rand_uniform, keyed by seed, step, tensor and element, so a step is
 // reproducible.  A v that is not zero is kept at the format's smallest value or above, never at zero: with
 // an m that is still there, zero would make the next update m / eps.  The update itself uses the moments
@@ -33,7 +34,7 @@ namespace slhip {
 constexpr int ADAMW_TENSORS = 64;   // of one launch: a lane each in the search for a workgroup's tensor
 constexpr int ADAMW_BLOCK = 256;    // elements of a scale: a wave's 64 lanes hold four each
 constexpr int ADAMW_ROWS = 2;       // blocks of 256 elements a wave takes (1, 2, 3, 4 of them: 134 M elements with 8-bit
-                                    // moments 362, 340, 345, 352 us, 40 M with f32 ones 189, 190, 197, 208)
+                                    // moments 370, 348, 350, 355 us, 5.8 M 19.7, 19.7, 20.2, 21.9, 40 M with f32 ones 188, 189, 196, 206)
 constexpr size_t ADAMW_TILE = (size_t)4 * ADAMW_ROWS * ADAMW_BLOCK;  // elements of a workgroup of four waves
 constexpr size_t ADAMW_LONGEST = MAX_GRID / ADAMW_TENSORS * ADAMW_TILE;  // elements of a tensor: 64 of them fit a launch
 
@@ -289,7 +290,8 @@ __global__ __launch_bounds__(256) void adamw8_kernel(Adamw8Args a) {
   }
 }
 
-// The arrays of a call, in the order of their addresses: 2^47 of those and 2^17 arrays make one 64-bit key.
+// The arrays of a call, in the order of their addresses: 2^47 of those and 2^17 arrays make one 64-bit key.  Sorting those takes 2 us for 64
+// tensors and 14 for 400 whose lists are in address order, 15 and 110 where they are in any order.
 constexpr size_t ADAMW_MOST = 16384;  // tensors of a call
 static_assert(5 * ADAMW_MOST + 1 <= (size_t(1) << 17), "arrays of a call");
 

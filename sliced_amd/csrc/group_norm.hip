@@ -15,8 +15,9 @@
 //            of their own, and the second kernel starts where the first one ended, with what the last-level cache still
 //            holds.
 //
-// Measured: 8192 rows x 2048 in 16 groups backward 44 us (4.6 TB/s), 32 x 1024 x 512 in 32 groups forward on chip 26 us (5.2
-// TB/s), 32 x 4096 x 512 in two passes forward 131 us (6.2 TB/s of the 12 bytes that those move), backward 240 (5.6 of 20).
+// Measured on inputs that change from call to call and exceed the last-level cache together: 8192 rows x 2048 in 16 groups backward 44
+// us (4.6 TB/s), as a layer norm forward 27 (5.0); 32 x 1024 x 512 in 32 groups forward on chip 34 us (4.0 TB/s), backward in two passes
+// 67; 32 x 4096 x 512 in two passes forward 131 us (6.1 TB/s of the 12 bytes that those move), backward 243 (5.5 of 20).
 //
 // In the latter two a window is a run of whole groups, about 32 vectors of channels wide (512 bytes of a row of x): narrower
 // pieces of rows than that cost HBM bandwidth.  Groups wider than a workgroup are cut.  A thread keeps to one vector of V
@@ -97,8 +98,10 @@ __device__ __forceinline__ NormVec<V> norm_param(const float* p, size_t c, float
 
 // What is left of a normal distribution beyond |u|, erfc(|u| / sqrt 2) / 2, and exp(-u^2 / 2), for x * Phi(x) and its slope.
 // erfc(x) is exp(-x^2) times a polynomial without constant in 1/(1 + 0.325 x): the form of Abramowitz and Stegun's formula
-// 7.1.26, three terms longer, its coefficients fitted here by reweighted least squares: 1.3e-8 off, and 2.6e-7 of itself
-// far out.  (The library's erff takes a branch each for small and large arguments, which both run in a wave; with it the
+// 7.1.26, three terms longer, its coefficients fitted here by reweighted least squares: in exact arithmetic 2.1e-8 off, and
+// 2.7e-7 of itself far out.  In 32 bits it is 1.9e-7 off near zero, and far out the rounding of the exponent's argument is what is
+// left: 4.6e-7 of itself at |u| = 2, 2.9e-6 at 8, 7e-6 at 12.  From |u| = 13.2 on, where exp(-u^2 / 2) leaves the normal floats, both are
+// zero.  (The library's erff takes a branch each for small and large arguments, which both run in a wave; with it the
 // arithmetic, not HBM, bounded these kernels: 10 x 961 x 390 forward 17 us.)
 __device__ __forceinline__ float norm_tail(float u, float& e) {
   const float t = __builtin_amdgcn_rcpf(fmaf(0.2298097014427185f, fabsf(u), 1.0f));

@@ -8,9 +8,10 @@
 // G_t = a_t d_t, so that a step needs its own gate only: d_t = dh_t + G_{t+1}, G_t = a_t d_t - the same recurrence
 // run from the last step to the first, with input a_t dh_t.
 //
-// HBM is the bound: 12 bytes an element forward, 20 (linear) or 24 (sigmoid) backward.  Measured: 32 x 1000 x 1024 forward
-// 73 us (5.4 TB/s), backward 152 (5.2); 8 x 2048 x 1024 forward 47 us (4.2), backward 88 (4.6); 65536 x 1024 linear 231 us
-// (5.8 TB/s of the 20 bytes that its split moves); 32 x 1 x 2048, a token, 2.8 us in the kernel.
+// HBM is the bound: 12 bytes an element forward, 20 (linear) or 24 (sigmoid) backward.  Measured on inputs that change from call
+// to call and exceed the last-level cache together, as all figures below unless they say otherwise: 32 x 1000 x 1024 forward 73 us (5.4
+// TB/s), backward 147 (5.4); 8 x 2048 x 1024 forward 46 us (4.4), backward 88 (4.6); 65536 x 1024 linear 232 us (5.8 TB/s of the 20 bytes
+// that its split moves), backward 316; 32 x 1 x 2048, a token, 2.8 us in the kernel.
 #include <type_traits>
 
 #include "common.hpp"
@@ -216,8 +217,8 @@ struct ScanRun {
 
 // Workgroups are dealt out to the 8 XCDs in turn; this numbers them so that each XCD gets a run of consecutive numbers.
 // Neighbouring channel tiles then share an L2, and the 128-byte lines that both have a part of are read and written once:
-// 64 x 1000 x 100 forward 19 us instead of 27, 4 x 4099 x 1001 backward 98 instead of 109.  Where no line is shared it
-// gains nothing and costs up to 5 % (65536 x 1024 linear 244 us, 233 without), so it is left out there.
+// 64 x 1000 x 100 forward 24 us instead of 30, 4 x 4099 x 1001 forward 69 instead of 75, backward 98 instead of 107.  Where no line is
+// shared it gains nothing and costs up to 4 % (65536 x 1024 linear 243 us, 233 without), so it is left out there.
 __device__ __forceinline__ unsigned scan_by_xcd(unsigned id, unsigned count) {
   const unsigned x = id & 7, each = count >> 3, more = count & 7;
   return x * each + (x < more ? x : more) + (id >> 3);
@@ -546,15 +547,15 @@ static int32_t scan_launch_tiles(slhip_ctx* ctx, const ScanArgs& a) {
 template <bool GRAD, int MODE>
 static int32_t scan_launch(slhip_ctx* ctx, const ScanArgs& a) {
   // steps of a run, and threads: forward longer runs and more of them, backward holds twice the arrays in registers
-  // (8 x 2048 x 1024: forward 4 and 512 41.4 us, 4 and 256 43.2, 2 and 512 41.5, which loses where steps are split; backward 2
-  // and 256 89.8 us, 2 and 512 91.9, 4 and 256 93.1)
+  // (8 x 2048 x 1024: forward 4 and 512 46.1 us, 4 and 256 48.2, 2 and 512 45.2, which loses where steps are split; backward 2
+  // and 256 87.4 us, 2 and 512 89.9, 4 and 256 90.5)
   constexpr int R = GRAD ? 2 : 4, NT = GRAD ? 256 : 512;
   if (a.steps > 8) {
     if (a.channels > 32) {
-      // Wide channel tiles, 512 bytes of a row, are what HBM likes best (32 x 1000 x 1024 backward: 151 us at 512 bytes, 167 at
-      // 256, 180 at 128; forward 74, 81, 92), if there are enough of them; narrow ones fill the chip where a split of the steps, which reads the
-      // inputs of the recurrence twice, would have to otherwise (forward 8 x 2048 x 1024 narrow 47 us, 4 x 4099 x 1024, which has
-      // as many elements and too few narrow tiles, wide and split 67).
+      // Wide channel tiles, 512 bytes of a row, are what HBM likes best (32 x 1000 x 1024 backward: 146 us at 512 bytes, 167 at
+      // 128; forward 73 and 84; 65536 x 1024 linear 232 and 269), if there are enough of them; narrow ones fill the chip where a split of the
+      // steps, which reads the inputs of the recurrence twice, would have to otherwise (forward 8 x 2048 x 1024 narrow 46 us, wide and
+      // split 68; 4 x 4099 x 1001 has too few narrow tiles too: wide 69, narrow 83, both split; backward 8 x 2048 x 1024 is level).
       const size_t cu = (size_t)ctx->num_cu, wide = a.batch * ((a.channels + 127) / 128), narrow = a.batch * ((a.channels + 31) / 32);
       if (a.channels > 64 && (wide >= cu || narrow < cu || a.steps < 256)) return scan_launch_tiles<GRAD, MODE, 4, 32, R, NT>(ctx, a);
       return scan_launch_tiles<GRAD, MODE, 4, 8, R, NT>(ctx, a);
