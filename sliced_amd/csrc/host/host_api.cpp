@@ -65,7 +65,7 @@ SLH_API int slh_device_ctx(void* dev, void** ctx) {  // the slhip context the de
 SLH_API int slh_record_begin(void* dev) {
   return guard([&] {
     HIP* d = (HIP*)dev;
-    d->run();
+    d->before_recording();
     check(slhip_graph_begin(d->ctx()), "slhip_graph_begin");
   });
 }

@@ -244,7 +244,7 @@ class HIP {
   // Graph is in use.
   template <class F>
   Graph record(F&& body) {
-    run();  // what was deferred before the recording belongs before it
+    before_recording();
     check(slhip_graph_begin(ctx_), "slhip_graph_begin");
     slhip_graph* g = nullptr;
     recording_ = true;
@@ -262,6 +262,17 @@ class HIP {
     recording_ = false;
     check(slhip_graph_end(ctx_, &g), "slhip_graph_end");
     return Graph(this, ctx_, g, std::move(recorded_seeds_));
+  }
+  // What was deferred before a recording belongs before it, the zero fills that zero_grad() left pending too: found by an op
+  // of the recording, a fill - or the op's overwriting in its place - would run in every replay, and replays that are to add up their
+  // gradients would not.  (A seed gradient that still holds its ones is left to backward().)
+  void before_recording() {
+    run();
+    const std::vector<uint64_t> pending(stale_.begin(), stale_.end());
+    for (uint64_t id : pending) {
+      auto it = allocs_.find(id);
+      if (it != allocs_.end() && !ones_.count(id)) settle(it->second);
+    }
   }
   // What a replay relies on without recording it: the host-side bookkeeping of zero_grad() and
   // backward() ran when the step was recorded, not now.  Every fill that is pending on the host

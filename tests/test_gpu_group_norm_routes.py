@@ -96,7 +96,7 @@ def smaller_workspace(c, size):
 @pytest.mark.parametrize("shape", [(7, 2500, 16, 4), (5, 3, 2600, 1), (40, 1, 96, 4), (6, 2200, 18, 3)])
 def test_samples_that_do_not_fit_the_workspace_at_once(hip, shape):
     """The two-pass kernels over three samples at a time and fewer at the end (and rows whose column sums do not fit, which take them
-    too): weights' and biases' gradients add up over the rounds, also onto what is there."""
+    too): weights' and biases' gradients add up over the launches, also onto what is there."""
     n, p, ch, g = shape
     x, w, b, dy = base.data(shape, SILU, tag=330)
     from sliced_amd.device import Context
@@ -142,7 +142,7 @@ def test_samples_that_do_not_fit_the_workspace_at_once(hip, shape):
             assert backward(beta) == 0
             for got, o, v, t, what in zip(outs, old, want, tol, ("x", "weight", "bias")):
                 v = v + beta * o.reshape(v.shape)
-                # (a round adds to what the one before left: four roundings of the sums at most)
+                # (a launch adds to what the one before left: four roundings of the sums at most)
                 base.close(got.numpy(), v, t + 4 * U * np.abs(v) + beta * 4 * U * np.abs(o.reshape(v.shape)), (what, beta))
         for only in range(3):
             outs[only].upload(np.full(outs[only].n, np.nan, np.float32))
